@@ -561,6 +561,67 @@ int ocean_clip_adam_step_auto(const ocean_adam_chunk* table, int n_chunks, ocean
                               const float* lr_dev, int* step_dev, float beta1, float beta2, float eps,
                               float weight_decay, int write_clipped, void* stream);
 
+/* ------------------------------------------------------------------ attention without stored weights
+ * No counterpart in the reference, whose ScaledDotProductAttention (multi_factor_attention.py:34-65) stores the weights
+ * [B, H, L, L].  out_i = sum_j p_ij v_j with p_i = softmax over the allowed keys j of scale * q_i . k_j (+ position bias); a
+ * query with no allowed key gets zeros.  Query i of sample b stands at position starts[b] + i (query_start + i without
+ * `starts`) among the keys.  Allowed: j < lengths[b] (clamped to 0..Lk; NULL: Lk), with causal j <= the query's position, and
+ * with a mask mask[b, h, i, j] != 0.  Keys and values past a sample's length are not read.  Query head h reads key head
+ * h / (H / Hk).  Positions are int32, |position| < 2^30.
+ * Position bias: table[bucket(j - position)][h] is added to the score.  With side = num_buckets (bidirectional: half of them for
+ * each sign, the upper half for keys after the query) and E = side / 2, distances n < E have a bucket each, farther ones share
+ * E + floor((side - E) ln(n / E) / ln(max_distance / E)), at most side - 1; one-sided, keys after the query count as n = 0.
+ * q, k, v, out and their gradients: dtype values, unit stride over the d features (4 or 8 (16 bits) <= d <= 128), strides in
+ * elements for batch, head, position (any; 0 = broadcast for inputs).  mask strides in bytes for b, h, i, j.
+ * lse [B, H, Lq] (may be NULL in the forward call): what the backward call needs besides the inputs and `out`.
+ * The backward call recomputes the probabilities; dq / dk / dv / dtable are overwritten, each may be NULL (dk / dv rows past a
+ * sample's length are zeros); sums run in a fixed order.  Workspaces in floats (0: none needed, or a bad shape). */
+#define OCEAN_F32 0
+#define OCEAN_BF16 1
+#define OCEAN_F16 2                /* layer norm only */
+typedef struct {
+  int B, H, Hk, Lq, Lk, d;
+  int dtype;
+  int causal;
+  int query_start;
+  float scale;                     /* > 0 */
+  int num_buckets;                 /* 0: no position bias; at most 128 */
+  int max_distance;                /* > E, at most 2048 */
+  int bidirectional;
+  long q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+  long go_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+  long mask_strides[4];
+} ocean_attention_shape;
+size_t ocean_attention_fwd_workspace(const ocean_attention_shape* s);
+size_t ocean_attention_bwd_workspace(const ocean_attention_shape* s);
+int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const void* k, const void* v, const uint8_t* mask,
+                        const int* lengths, const int* starts, const float* table /* [num_buckets, H] */, float* ws,
+                        size_t ws_floats, void* out, float* lse, void* stream);
+int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const void* k, const void* v, const uint8_t* mask,
+                        const int* lengths, const int* starts, const float* table, const void* out, const float* lse,
+                        const void* d_out, float* ws, size_t ws_floats, void* dq, void* dk, void* dv, float* dtable,
+                        void* stream);
+
+/* ------------------------------------------------------------------ layer norm of rows of any width
+ * No entry of the reference (nn.LayerNorm inside its modules).  y = (x - mean) / sqrt(var + eps) * weight + bias over `width`
+ * values; with `residual`, x + residual is rounded to dtype, written to `sum` and normalised.  x, residual, dy, d_sum: rows at
+ * the given strides (elements); y, sum, dx: dense rows; weight / bias fp32 or NULL; stats [rows][2] (mean, 1 / deviation; may
+ * be NULL in the forward call) is what the backward call needs.  Backward: x is the normalised input (`sum` with a residual);
+ * dx = gradient through the norm (+ d_sum), overwritten, the same for x and residual; dweight / dbias fp32, overwritten, summed
+ * in a fixed order.  dx, dweight, dbias, d_sum may be NULL; ws is needed for dweight / dbias. */
+typedef struct {
+  long rows;
+  int width;
+  int dtype;
+  float eps;
+  long x_stride, residual_stride, dy_stride, dsum_stride;
+} ocean_layer_norm_shape;
+int ocean_layer_norm_fwd(const ocean_layer_norm_shape* s, const void* x, const void* residual, const float* weight,
+                         const float* bias, void* y, void* sum, float* stats, void* stream);
+size_t ocean_layer_norm_bwd_workspace(const ocean_layer_norm_shape* s);
+int ocean_layer_norm_bwd(const ocean_layer_norm_shape* s, const void* x, const float* stats, const float* weight, const void* dy,
+                         const void* d_sum, float* ws, size_t ws_floats, void* dx, float* dweight, float* dbias, void* stream);
+
 /* ------------------------------------------------------------------ kernel timing (measurement aid)
  * No counterpart in the reference.  While enabled, every GEMM launch is bracketed by HIP events on its
  * stream (this is the one place the library creates runtime objects).  ocean_prof_summary waits for the

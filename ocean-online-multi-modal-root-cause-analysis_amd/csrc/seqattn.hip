@@ -1,0 +1,122 @@
+// Entry points of attention without stored weights: argument checks, launch plan, workspaces.
+#include "seqattn.h"
+
+namespace {
+
+using seqattn::Params;
+using seqattn::View;
+
+View view(const void* p, const long* st) { View v; v.p = p; v.b = st[0]; v.h = st[1]; v.l = st[2]; return v; }
+
+// the buckets' limits in whole numbers: far bucket exact + k begins at the smallest n >= exact with
+// (n / exact)^far >= (max_distance / exact)^k, that is far * ln(n / exact) >= k * ln(max_distance / exact).  In fp64 the two
+// sides of an equality differ by a few 1e-16, two different ones by more than 1e-6 (n < 2^12): the slack decides ties.
+void bucket_limits(Params& p) {
+  const double span = log((double)p.max_dist / p.exact);
+  const int far = p.side - p.exact;
+  int n = p.exact;
+  for (int k = 1; k < far; ++k) {
+    while (n < p.max_dist && far * log((double)n / p.exact) < k * span - 1e-9) ++n;
+    p.limits[k - 1] = n;
+  }
+}
+
+struct Plan { int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, parts_at; };
+
+int plan_of(const ocean_attention_shape* s, Plan* pl) {
+  if (!s) return OCEAN_ERR_NULL;
+  if (s->B <= 0 || s->H <= 0 || s->Hk <= 0 || s->Lq <= 0 || s->Lk <= 0 || s->d <= 0 || s->H % s->Hk != 0) return OCEAN_ERR_BAD_SHAPE;
+  if (s->dtype != OCEAN_F32 && s->dtype != OCEAN_BF16) return OCEAN_ERR_BAD_SHAPE;
+  if (!(s->scale > 0.f) || s->scale > 3.0e38f) return OCEAN_ERR_BAD_SHAPE;
+  if (s->d < (s->dtype == OCEAN_F32 ? 4 : 8) || s->d > 128) return OCEAN_ERR_UNSUPPORTED;
+  if (s->Lq > (1 << 30) || s->Lk > (1 << 30) || s->query_start > (1 << 30) || s->query_start < -(1 << 30)) return OCEAN_ERR_UNSUPPORTED;
+  const int G = s->H / s->Hk;
+  if ((long)s->Lq * G > (1L << 30)) return OCEAN_ERR_UNSUPPORTED;
+  if (s->num_buckets != 0) {
+    const int side = s->bidirectional ? s->num_buckets / 2 : s->num_buckets;
+    if (s->num_buckets < 0 || (s->bidirectional && s->num_buckets % 2) || side < 2 || s->max_distance <= side / 2) return OCEAN_ERR_BAD_SHAPE;
+    if (s->num_buckets > seqattn::kMaxBuckets || s->max_distance > seqattn::kMaxDist) return OCEAN_ERR_UNSUPPORTED;
+  }
+  pl->D = (s->d + 31) / 32 * 32;
+  const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
+  if (blocks > 0x7fffffffL || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;
+  // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as rows.
+  pl->split = (long)s->Lq * G <= 32;
+  pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
+  const long base = (long)s->B * s->Hk * pl->chunks;
+  long want = (512 + base - 1) / base;
+  const long most = (s->Lk + 255) / 256;
+  if (want > most) want = most;
+  pl->splits = (int)(want < 1 ? 1 : want);
+  if (base * pl->splits > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;
+  pl->fwd_floats = pl->split && pl->splits > 1 ? (size_t)base * pl->splits * 32 * (pl->D + 2) : 0;
+  const size_t rows = (size_t)s->B * s->H * s->Lq;
+  pl->parts_at = (rows + 3) & ~size_t(3);
+  pl->bwd_floats = pl->parts_at + (size_t)s->B * s->H * ((s->Lk + 127) / 128) * (s->num_buckets > 0 ? s->num_buckets : 0);
+  return OCEAN_OK;
+}
+
+int fill(const ocean_attention_shape* s, const Plan& pl, const void* q, const void* k, const void* v, const uint8_t* mask, const int* lengths,
+         const int* starts, const float* table, Params* out) {
+  if (!q || !k || !v) return OCEAN_ERR_NULL;
+  if ((s->num_buckets > 0) != (table != nullptr)) return OCEAN_ERR_NULL;
+  Params& p = *out;
+  p = Params{};
+  p.q = view(q, s->q_strides); p.k = view(k, s->k_strides); p.v = view(v, s->v_strides);
+  p.B = s->B; p.H = s->H; p.Hk = s->Hk; p.G = s->H / s->Hk; p.Lq = s->Lq; p.Lk = s->Lk; p.d = s->d; p.scale = s->scale; p.causal = s->causal != 0;
+  p.start0 = s->query_start; p.lengths = lengths; p.starts = starts;
+  p.mask = mask; p.mb = s->mask_strides[0]; p.mh = s->mask_strides[1]; p.mi = s->mask_strides[2]; p.mj = s->mask_strides[3];
+  p.table = table; p.buckets = s->num_buckets; p.both = s->bidirectional != 0; p.max_dist = s->max_distance;
+  if (table) {
+    p.side = p.both ? p.buckets / 2 : p.buckets;
+    p.exact = p.side / 2;
+    bucket_limits(p);
+  }
+  p.q_tiles = (s->Lq + 127) / 128;
+  return OCEAN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ocean_attention_fwd_workspace(const ocean_attention_shape* s) { Plan pl; return plan_of(s, &pl) == OCEAN_OK ? pl.fwd_floats : 0; }
+size_t ocean_attention_bwd_workspace(const ocean_attention_shape* s) { Plan pl; return plan_of(s, &pl) == OCEAN_OK ? pl.bwd_floats : 0; }
+
+int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const void* k, const void* v, const uint8_t* mask, const int* lengths,
+                        const int* starts, const float* table, float* ws, size_t ws_floats, void* out, float* lse, void* stream) {
+  Plan pl;
+  Params p;
+  OCEAN_TRY(plan_of(s, &pl));
+  OCEAN_TRY(fill(s, pl, q, k, v, mask, lengths, starts, table, &p));
+  if (!out || (pl.fwd_floats && !ws)) return OCEAN_ERR_NULL;
+  if (ws_floats < pl.fwd_floats) return OCEAN_ERR_WORKSPACE;
+  p.o = view(out, s->o_strides);
+  p.lse = lse;
+  if (pl.split) {
+    p.splits = pl.splits;
+    p.q_tiles = pl.chunks;
+    const size_t rows = (size_t)s->B * s->Hk * pl.chunks * pl.splits * 32;
+    p.part_o = ws;
+    p.part_ml = ws + rows * pl.D;
+  }
+  return seqattn::launch_forward(p, s->dtype, (hipStream_t)stream);
+}
+
+int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const void* k, const void* v, const uint8_t* mask, const int* lengths,
+                        const int* starts, const float* table, const void* out, const float* lse, const void* d_out, float* ws, size_t ws_floats,
+                        void* dq, void* dk, void* dv, float* dtable, void* stream) {
+  Plan pl;
+  Params p;
+  OCEAN_TRY(plan_of(s, &pl));
+  OCEAN_TRY(fill(s, pl, q, k, v, mask, lengths, starts, table, &p));
+  if (!out || !lse || !d_out || !ws || (dtable && !table)) return OCEAN_ERR_NULL;
+  if (ws_floats < pl.bwd_floats) return OCEAN_ERR_WORKSPACE;
+  p.o = view(out, s->o_strides); p.go = view(d_out, s->go_strides); p.lse = const_cast<float*>(lse);
+  p.dq = view(dq, s->dq_strides); p.dk = view(dk, s->dk_strides); p.dv = view(dv, s->dv_strides);
+  p.delta = ws;
+  p.dtable_part = dtable ? ws + pl.parts_at : nullptr;
+  return seqattn::launch_backward(p, s->dtype, dtable, (hipStream_t)stream);
+}
+
+}  // extern "C"

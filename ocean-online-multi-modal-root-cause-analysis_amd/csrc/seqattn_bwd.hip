@@ -1,0 +1,387 @@
+// Backward pass of attention without stored weights (seqattn.h).  With the row's log-sum from the forward pass,
+//   p_ij = 2^(s_ij - lse_i),  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i),  delta_i = do_i . o_i,
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,   dbias(dist) = sum of ds over a diagonal.
+// Two launches, each of which owns what it sums: one over queries (dq, delta), one over keys (dk, dv, with the heads that share
+// a key head as more rows of the sum, and the bias).  The scores are formed in both - seven products instead of five - and in
+// exchange no gradient is summed by atomics or through memory: results do not depend on the order of the blocks.
+#include "seqattn.h"
+
+namespace seqattn {
+namespace {
+
+constexpr int kRows = 128;           // queries (keys) of a block: four waves, 32 each
+
+// p_ij for keys j0.. of this lane's query, from scores
+template <bool BIAS> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int keys,
+                                                                   const uint8_t* mrow, const float* lut, bool edge, int lane) {
+  const int h4 = 4 * (lane >> 5);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float t = BIAS ? lut[dist_slot(p, j0 + 8 * (r >> 2) + h4 + (r & 3) - pos)] - lse : -lse;
+    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
+  }
+  if (edge) {
+    const int end = p.causal ? min(keys, pos + 1) : keys;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int j = j0 + 8 * g + h4;
+      const uint32_t ok = mrow ? mask4(p, mrow, j, keys) : 15u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) if (j + e >= end || !((ok >> e) & 1u)) s[4 * g + e] = 0.f;
+    }
+  }
+}
+
+// Sums of a wave's 32x32 block of ds (rows: queries, own columns: keys) over its 63 diagonals, through LDS of the wave (pitch
+// 33: a diagonal is a fixed step), lane t taking distance d0 + t - 31; then into the wave's own sums by distance.  One lane owns one distance, and blocks follow
+// each other in order: the sums come out the same in every run.
+struct DiagSums {
+  float* scratch;                    // [32][33]
+  float* by_dist;                    // [2 max_dist + 1]
+  float below, above;                // distances of -max_dist and less, max_dist and more
+  __device__ __forceinline__ void add(const Params& p, const f32x16& ds, int d0, int lane) {
+    if (d0 + 31 <= -p.max_dist || d0 - 31 >= p.max_dist) {
+      float t = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t += ds[r];
+      if (d0 < 0) below += t; else above += t;
+      return;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * 33 + (lane & 31)] = ds[r];
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int j = i + lane - 31;
+      const float x = scratch[i * 33 + min(max(j, 0), 31)];
+      t += j >= 0 && j < 32 ? x : 0.f;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int dist = d0 + lane - 31;
+    if (dist <= -p.max_dist) below += t;
+    else if (dist >= p.max_dist) above += t;
+    else if (lane < 63) by_dist[dist + p.max_dist] += t;
+  }
+};
+
+// the block's sums by bucket (each bucket a run of distances), and the sums by distance back to zero for the next head
+__device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag, float* dist_sums, float* part, int tid) {
+  const int slots = 2 * p.max_dist + 1;
+  float lo = diag.below, hi = diag.above;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { lo += __shfl_xor(lo, o, 64); hi += __shfl_xor(hi, o, 64); }
+  if ((tid & 63) == 0) { diag.by_dist[0] += lo; diag.by_dist[slots - 1] += hi; }
+  diag.below = diag.above = 0.f;
+  __syncthreads();
+  for (int k = tid; k < p.buckets; k += 256) {
+    // bucket k holds the distances of n0..n1 steps to one side
+    const int right = p.both && k >= p.side, f = right ? k - p.side : k;
+    int n0 = f <= p.exact ? f : p.limits[f - p.exact - 1];
+    const int n1 = f == p.side - 1 ? p.max_dist : f < p.exact ? f : p.limits[f - p.exact] - 1;
+    int x0 = p.max_dist - n1, x1 = p.max_dist - n0;
+    if (right) { n0 = max(n0, 1); x0 = p.max_dist + n0; x1 = p.max_dist + n1; }
+    if (!p.both && f == 0) x1 = slots - 1;
+    float t = 0.f;
+    for (int x = x0; x <= x1; ++x)
+      for (int v = 0; v < 4; ++v) t += dist_sums[v * slots + x];
+    part[k] = t;
+  }
+  __syncthreads();
+  for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
+  __syncthreads();
+}
+
+template <typename T, int D> struct BwdTile { static constexpr int kRows = sizeof(T) == 2 ? 64 : 32; };
+
+template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void dq_kernel(const Params p) {
+  typedef Tile<T, D> TL;
+  constexpr int BN = BwdTile<T, D>::kRows, NS = BN / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int kBuf = BN * TL::kRowBytes;                  // two buffers of keys, two of values
+  char* const kt = smem;
+  char* const vt = smem + 2 * kBuf;
+  float* const lut = reinterpret_cast<float*>(smem + 4 * BN * TL::kRowBytes);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int id = die_order(blockIdx.x, gridDim.x);
+  const int tile = p.q_tiles - 1 - id % p.q_tiles, bh = id / p.q_tiles, b = bh / p.H, head = bh % p.H, kh = head / p.G;
+  const int keys = keys_of(p, b), start = start_of(p, b);
+  const int i0 = tile * kRows + 32 * w, i = i0 + (lane & 31), pos = start + i;
+  const bool live = i < p.Lq;
+  if (BIAS) fill_bias(p, head, lut, tid, 256);
+  const T* kb = (const T*)p.k.p + b * p.k.b + kh * p.k.h;
+  const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
+  RowRegs<T, D> q, go;
+  q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
+  go.load(live ? (const T*)p.go.p + b * p.go.b + head * p.go.h + (long)i * p.go.l : nullptr, p.d, lane);
+  float delta = 0.f, lse = INFINITY;
+  if (live) {
+    RowRegs<T, D> o;
+    o.load((const T*)p.o.p + b * p.o.b + head * p.o.h + (long)i * p.o.l, p.d, lane);
+#pragma unroll
+    for (int s = 0; s < RowRegs<T, D>::kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < Mm<T>::kEpc; ++e) delta = fmaf((float)go.f[s][e], (float)o.f[s][e], delta);
+    lse = p.lse[((long)b * p.H + head) * p.Lq + i];
+  }
+  delta = other_half_sum(delta);
+  float rest = 0.f;
+  const uint8_t* mrow = p.mask && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
+  int end = keys, wend = keys, wfull = keys;
+  if (p.causal) {
+    end = min(end, start + min(tile * kRows + kRows, p.Lq));
+    wend = min(wend, start + min(i0 + 32, p.Lq));
+    wfull = min(wfull, start + i0 + 1);
+  }
+  const float c = p.scale * kLog2e;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
+  Stage<T, D, BN, 256> ks, vs;
+  const int tiles = end > 0 ? (end + BN - 1) / BN : 0;
+  if (tiles > 0) {
+    ks.fetch(kb, p.k.l, 0, keys, p.d, tid);
+    vs.fetch(vb, p.v.l, 0, keys, p.d, tid);
+    ks.put(kt, tid);
+    vs.put(vt, tid);
+  }
+  // Up to two tiles of keys sit in the two buffers.  Rows of so few keys are where 16-bit rounding of `o` reaches dq through delta
+  // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first.
+  const bool few = sizeof(T) == 2 && tiles <= 2;
+  if (few && tiles == 2) {
+    ks.fetch(kb, p.k.l, BN, keys, p.d, tid);
+    vs.fetch(vb, p.v.l, BN, keys, p.d, tid);
+    ks.put(kt + kBuf, tid);
+    vs.put(vt + kBuf, tid);
+  }
+  __syncthreads();
+  if (few) {
+    float sum = 0.f;
+    for (int j = 0; j < wend; j += 32) {
+      const int at = j / BN * kBuf, row = j % BN;
+      f32x16 s = row_mma<T, D>(kt + at, row, lane, q, f32x16{});
+      const f32x16 dp = row_mma<T, D>(vt + at, row, lane, go, f32x16{});
+      probabilities<BIAS>(p, s, c, lse, j, pos, keys, mrow, lut, p.mask || j + 32 > wfull, lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum = fmaf(s[r], dp[r], sum);
+    }
+    delta = other_half_sum(sum);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    const int j0 = t * BN, cur = t & 1;
+    const bool more = t + 1 < tiles && !few;
+    if (more) {
+      ks.fetch(kb, p.k.l, j0 + BN, keys, p.d, tid);
+      vs.fetch(vb, p.v.l, j0 + BN, keys, p.d, tid);
+    }
+    if (j0 < wend) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const int j = j0 + 32 * n;
+        f32x16 s = row_mma<T, D>(kt + cur * kBuf, 32 * n, lane, q, f32x16{});
+        const f32x16 dp = row_mma<T, D>(vt + cur * kBuf, 32 * n, lane, go, f32x16{});
+        probabilities<BIAS>(p, s, c, lse, j, pos, keys, mrow, lut, p.mask || j + 32 > wfull, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] *= dp[r] - delta;
+          if (sizeof(T) == 2) rest += s[r];
+        }
+        PFrag<T> pf;
+        pf.set(s);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) acc[db] = col_mma<D>(kt + cur * kBuf, 32 * n, db, lane, pf, acc[db]);
+      }
+    }
+    if (more) {
+      ks.put(kt + (cur ^ 1) * kBuf, tid);
+      vs.put(vt + (cur ^ 1) * kBuf, tid);
+    }
+    __syncthreads();
+  }
+  if (live && p.dq.p) store_row<T, D>((T*)p.dq.p + b * p.dq.b + head * p.dq.h + (long)i * p.dq.l, acc, p.scale, p.d, lane);
+  // In 16 bits `o` was rounded, and so were the weights that formed it: delta is a few 1e-3 of |do| |o| off.  The row's ds sum to
+  // what is missing, in fp32 and for one addition each; the launch over keys, and the bias with it, gets the exact delta.
+  if (sizeof(T) == 2) delta += other_half_sum(rest);
+  if (live && lane < 32) p.delta[((long)b * p.H + head) * p.Lq + i] = delta;
+}
+
+template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void dkv_kernel(const Params p, const int k_tiles) {
+  typedef Tile<T, D> TL;
+  constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int kBuf = BM * TL::kRowBytes;                  // two buffers of queries, two of the outputs' gradients
+  char* const qt = smem;
+  char* const gt = smem + 2 * kBuf;
+  float* const rowv = reinterpret_cast<float*>(smem + 4 * BM * TL::kRowBytes);      // [2][lse, delta][BM]
+  float* const lut = rowv + 4 * BM;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h4 = 4 * (lane >> 5), slots = 2 * p.max_dist + 1;
+  DiagSums diag;
+  float* const dist_sums = lut + slots;                     // [wave][slots], then the waves' scratch
+  const bool sum_bias = BIAS && p.dtable_part != nullptr;
+  if (BIAS) {
+    diag.by_dist = dist_sums + w * slots;
+    diag.scratch = dist_sums + 4 * slots + w * 32 * 33;
+    diag.below = diag.above = 0.f;
+    if (sum_bias) for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
+  }
+  const int id = die_order(blockIdx.x, gridDim.x);
+  const int tile = id % k_tiles, bk = id / k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
+  const int keys = keys_of(p, b), start = start_of(p, b);
+  const int j0 = tile * kRows + 32 * w, j = j0 + (lane & 31);
+  const bool live = j < keys;
+  RowRegs<T, D> k, v;
+  k.load(live ? (const T*)p.k.p + b * p.k.b + kh * p.k.h + (long)j * p.k.l : nullptr, p.d, lane);
+  v.load(live ? (const T*)p.v.p + b * p.v.b + kh * p.v.h + (long)j * p.v.l : nullptr, p.d, lane);
+  const float c = p.scale * kLog2e;
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) { dk[db] = f32x16{}; dv[db] = f32x16{}; }
+  // queries from `first` on see some key of the block (of this wave); from `full` on all keys of this wave
+  int first = 0, wfirst = 0, wfull = 0;
+  if (p.causal) {
+    first = min(max(tile * kRows - start, 0), p.Lq);
+    wfirst = max(j0 - start, 0);
+    wfull = j0 + 31 - start;
+  }
+  if (tile * kRows >= keys) first = p.Lq;
+  const int t0 = first / BM, tiles = (p.Lq + BM - 1) / BM - t0, all = tiles * p.G;
+  const int head0 = kh * p.G;
+  Stage<T, D, BM, 256> qs, gs;
+  float rv = 0.f;                                           // threads 0..BM-1: lse, BM..2BM-1: delta
+  const auto fetch = [&](int u) {
+    const int head = head0 + u / tiles, r0 = (t0 + u % tiles) * BM;
+    qs.fetch((const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
+    gs.fetch((const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
+    if (tid < 2 * BM) {
+      const int i = r0 + tid % BM;
+      const bool in = i < p.Lq;
+      const float* from = tid < BM ? p.lse : p.delta;
+      rv = in ? from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? INFINITY : 0.f;
+    }
+  };
+  const auto put = [&](int cur) {
+    qs.put(qt + cur * kBuf, tid);
+    gs.put(gt + cur * kBuf, tid);
+    if (tid < 2 * BM) rowv[cur * 2 * BM + tid] = rv;
+  };
+  if (all > 0) { fetch(0); put(0); }
+  if (BIAS && all > 0) fill_bias(p, head0, lut, tid, 256);
+  __syncthreads();
+  for (int u = 0; u < all; ++u) {
+    const int cur = u & 1, g = u / tiles, head = head0 + g, r0 = (t0 + u % tiles) * BM;
+    if (BIAS && u > 0 && u % tiles == 0) {
+      fill_bias(p, head, lut, tid, 256);
+      __syncthreads();
+    }
+    if (u + 1 < all) fetch(u + 1);
+    if (j0 < keys && r0 + BM > wfirst) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const int i0 = r0 + 32 * n;
+        const float* lr = rowv + cur * 2 * BM + 32 * n + h4;
+        f32x16 s = row_mma<T, D>(qt + cur * kBuf, 32 * n, lane, k, f32x16{});
+        const f32x16 dp = row_mma<T, D>(gt + cur * kBuf, 32 * n, lane, v, f32x16{});
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int at = 8 * (r >> 2) + (r & 3);
+          const float t = BIAS ? lut[dist_slot(p, j - (start + i0 + h4 + at))] - lr[at] : -lr[at];
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
+        }
+        if (p.mask || j0 + 32 > keys || (p.causal && i0 < wfull)) {
+          const uint8_t* mcol = p.mask ? p.mask + b * p.mb + head * p.mh + (long)j * p.mj : nullptr;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int i = i0 + h4 + 8 * (r >> 2) + (r & 3);
+            bool ok = live && !(p.causal && j > start + i);
+            if (mcol && ok && i < p.Lq) ok = mcol[(long)i * p.mi] != 0;
+            if (!ok) s[r] = 0.f;
+          }
+        }
+        PFrag<T> pf;
+        pf.set(s);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) dv[db] = col_mma<D>(gt + cur * kBuf, 32 * n, db, lane, pf, dv[db]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= dp[r] - lr[BM + 8 * (r >> 2) + (r & 3)];
+        if (sum_bias) diag.add(p, s, j0 - (start + i0), lane);
+        pf.set(s);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) dk[db] = col_mma<D>(qt + cur * kBuf, 32 * n, db, lane, pf, dk[db]);
+      }
+    }
+    if (u + 1 < all) put(cur ^ 1);
+    __syncthreads();
+    if (sum_bias && u % tiles == tiles - 1) store_bias_sums(p, diag, dist_sums, p.dtable_part + (((long)head * p.B + b) * k_tiles + tile) * p.buckets, tid);
+  }
+  if (sum_bias && all == 0)
+    for (int x = tid; x < p.G * p.buckets; x += 256) p.dtable_part[(((long)(head0 + x / p.buckets) * p.B + b) * k_tiles + tile) * p.buckets + x % p.buckets] = 0.f;
+  if (j < p.Lk) {                                           // keys past the sample's end get zeros
+    if (p.dk.p) store_row<T, D>((T*)p.dk.p + b * p.dk.b + kh * p.dk.h + (long)j * p.dk.l, dk, p.scale, p.d, lane);
+    if (p.dv.p) store_row<T, D>((T*)p.dv.p + b * p.dv.b + kh * p.dv.h + (long)j * p.dv.l, dv, 1.f, p.d, lane);
+  }
+}
+
+// dtable[bucket][head]: the blocks' sums in their order, in 64 bits
+__global__ __launch_bounds__(256) void dtable_kernel(const float* __restrict__ part, float* __restrict__ out, int blocks, int buckets, int H) {
+  __shared__ double red[256];
+  const int head = blockIdx.x, k = blockIdx.y;
+  double t = 0.0;
+  for (int n = threadIdx.x; n < blocks; n += 256) t += part[((long)head * blocks + n) * buckets + k];
+  red[threadIdx.x] = t;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[(long)k * H + head] = (float)red[0];
+}
+
+template <typename K> int set_lds(K kernel, size_t bytes) {
+  if (bytes <= 65536) return OCEAN_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
+}
+
+template <typename T, int D, bool BIAS> int backward(const Params& p, float* dtable, hipStream_t s) {
+  typedef Tile<T, D> TL;
+  constexpr int BN = BwdTile<T, D>::kRows;
+  const size_t slots = 2 * p.max_dist + 1;
+  size_t lds = 4 * BN * TL::kRowBytes;
+  if (BIAS) lds += slots * sizeof(float);
+  OCEAN_TRY(set_lds(dq_kernel<T, D, BIAS>, lds));
+  hipLaunchKernelGGL((dq_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
+  OCEAN_LAUNCH_CHECK();
+  const int k_tiles = (p.Lk + kRows - 1) / kRows;
+  if (p.dk.p || p.dv.p || p.dtable_part) {
+    lds = 4 * BN * TL::kRowBytes + 4 * BN * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
+    if (BIAS && p.dtable_part) lds += (4 * slots + 4 * 32 * 33) * sizeof(float);
+    OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS>, lds));
+    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.Hk * k_tiles)), dim3(256), lds, s, p, k_tiles);
+    OCEAN_LAUNCH_CHECK();
+  }
+  if (BIAS && p.dtable_part) {
+    hipLaunchKernelGGL(dtable_kernel, dim3(p.H, p.buckets), dim3(256), 0, s, p.dtable_part, dtable, p.B * k_tiles, p.buckets, p.H);
+    OCEAN_LAUNCH_CHECK();
+  }
+  return OCEAN_OK;
+}
+
+template <typename T, int D> int backward_b(const Params& p, float* dtable, hipStream_t s) {
+  return p.table ? backward<T, D, true>(p, dtable, s) : backward<T, D, false>(p, dtable, s);
+}
+template <typename T> int backward_d(const Params& p, float* dtable, hipStream_t s) {
+  if (p.d <= 32) return backward_b<T, 32>(p, dtable, s);
+  if (p.d <= 64) return backward_b<T, 64>(p, dtable, s);
+  if (p.d <= 96) return backward_b<T, 96>(p, dtable, s);
+  return backward_b<T, 128>(p, dtable, s);
+}
+
+}  // namespace
+
+int launch_backward(const Params& p, int type, float* dtable, hipStream_t s) {
+  return type == OCEAN_BF16 ? backward_d<__bf16>(p, dtable, s) : backward_d<float>(p, dtable, s);
+}
+
+}  // namespace seqattn

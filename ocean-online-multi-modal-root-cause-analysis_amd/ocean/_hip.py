@@ -122,6 +122,18 @@ class GatConvShape(ctypes.Structure):
                 ("negative_slope", c_float), ("dropout", c_float), ("seed", c_uint64), ("seed_epoch", c_void_p)]
 
 
+class AttentionShape(ctypes.Structure):
+    _fields_ = [("B", c_int), ("H", c_int), ("Hk", c_int), ("Lq", c_int), ("Lk", c_int), ("d", c_int), ("dtype", c_int),
+                ("causal", c_int), ("query_start", c_int), ("scale", c_float), ("num_buckets", c_int), ("max_distance", c_int),
+                ("bidirectional", c_int)] + [(n + "_strides", c_long * 3) for n in ("q", "k", "v", "o", "go", "dq", "dk", "dv")] + [
+                ("mask_strides", c_long * 4)]
+
+
+class LayerNormShape(ctypes.Structure):
+    _fields_ = [("rows", c_long), ("width", c_int), ("dtype", c_int), ("eps", c_float), ("x_stride", c_long),
+                ("residual_stride", c_long), ("dy_stride", c_long), ("dsum_stride", c_long)]
+
+
 class AdamChunk(ctypes.Structure):
     _fields_ = [("param", c_uint64), ("grad", c_uint64), ("exp_avg", c_uint64), ("exp_avg_sq", c_uint64),
                 ("n", ctypes.c_int64)]
@@ -184,6 +196,15 @@ def _declare_rest(lib) -> None:
     sig("ocean_gatconv_bwd_workspace", c_size_t, gp_)
     sig("ocean_gatconv_fwd", c_int, gp_, vp, tp, tp, vp, c_size_t, vp, vp)
     sig("ocean_gatconv_bwd", c_int, gp_, vp, tp, tp, vp, vp, vp, c_size_t, tp, vp, vp)
+    at_ = POINTER(AttentionShape)
+    sig("ocean_attention_fwd_workspace", c_size_t, at_)
+    sig("ocean_attention_bwd_workspace", c_size_t, at_)
+    sig("ocean_attention_fwd", c_int, at_, vp, vp, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp)
+    sig("ocean_attention_bwd", c_int, at_, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp, vp, vp)
+    ln_ = POINTER(LayerNormShape)
+    sig("ocean_layer_norm_fwd", c_int, ln_, vp, vp, vp, vp, vp, vp, vp, vp)
+    sig("ocean_layer_norm_bwd_workspace", c_size_t, ln_)
+    sig("ocean_layer_norm_bwd", c_int, ln_, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp, vp)
     sig("ocean_bce_fwd", c_int, vp, vp, c_long, c_long, vp, vp)
     sig("ocean_bce_bwd", c_int, vp, vp, vp, c_long, c_long, vp, vp)
     sig("ocean_conv_gemm_f32", c_int, vp, c_int, vp, c_int, vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_long, c_long, c_int, vp)

@@ -6,10 +6,14 @@ stream.  None of them has a CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from typing import Optional
+import math
+from typing import Optional, Tuple, Union
 
 import torch
+
+from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -373,3 +377,283 @@ def diversity_loss(x: torch.Tensor) -> torch.Tensor:
     if x.dim() != 2:
         raise ValueError("expected [batch, dim]")
     return _Diversity.apply(x.contiguous().float())
+
+
+# ---------------------------------------------------------------- sequences: attention without stored weights, layer norm
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on(device):
+    """The device guard of the sequence operators: their tensors may live on another GPU than the current one."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _gpu(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+    if not t.is_cuda:
+        raise _hip.OceanHipError(f"{name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} lives on {t.device}, the other inputs on {like.device}")
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor in t's memory order, features innermost."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
+def _set_strides(field, t: torch.Tensor) -> None:
+    field[0], field[1], field[2] = t.stride(0), t.stride(1), t.stride(2)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, lengths, starts, table, causal, start, scale, max_distance, both):
+        L = _hip.lib()
+        sh = _hip.AttentionShape()
+        sh.B, sh.H, sh.Lq, sh.d = q.shape
+        sh.Hk, sh.Lk = k.shape[1], k.shape[2]
+        sh.dtype, sh.causal, sh.query_start, sh.scale = _DTYPES[q.dtype], causal, start, scale
+        _set_strides(sh.q_strides, q)
+        _set_strides(sh.k_strides, k)
+        _set_strides(sh.v_strides, v)
+        if mask is not None:
+            for n, st in enumerate(mask.stride()):
+                sh.mask_strides[n] = st
+        if table is not None:
+            sh.num_buckets, sh.max_distance, sh.bidirectional = table.shape[0], max_distance, both
+        out = _like(q)
+        _set_strides(sh.o_strides, out)
+        ctx.sh = sh
+        if q.numel() == 0 or k.numel() == 0:
+            ctx.save_for_backward(q, k, v, table)
+            return out.zero_()
+        train = any(ctx.needs_input_grad)
+        with _on(q.device):
+            lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32) if train else None
+            n = L.ocean_attention_fwd_workspace(ctypes.byref(sh))
+            ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+            _hip.check(L.ocean_attention_fwd(ctypes.byref(sh), _at(q), _at(k), _at(v), _at(mask), _at(lengths), _at(starts), _at(table),
+                                             _at(ws), n, _at(out), _at(lse), _hip.stream()), "ocean_attention_fwd")
+        if train:
+            ctx.save_for_backward(q, k, v, table, mask, lengths, starts, out, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        L = _hip.lib()
+        sh = ctx.sh
+        need = [ctx.needs_input_grad[n] for n in (0, 1, 2, 6)]
+        if len(ctx.saved_tensors) == 4:                       # no query or no key: nothing depends on anything
+            g = [torch.zeros_like(t) if n else None for n, t in zip(need, ctx.saved_tensors)]
+        else:
+            q, k, v, table, mask, lengths, starts, out, lse = ctx.saved_tensors
+            if d_out.stride(3) != 1:
+                d_out = d_out.contiguous()
+            g = [_like(t) if n else None for n, t in zip(need, (q, k, v, table))]
+            _set_strides(sh.go_strides, d_out)
+            for field, t in zip((sh.dq_strides, sh.dk_strides, sh.dv_strides), g):
+                if t is not None:
+                    _set_strides(field, t)
+            with _on(q.device):
+                ws = torch.empty(L.ocean_attention_bwd_workspace(ctypes.byref(sh)), device=q.device, dtype=torch.float32)
+                _hip.check(L.ocean_attention_bwd(ctypes.byref(sh), _at(q), _at(k), _at(v), _at(mask), _at(lengths), _at(starts), _at(table),
+                                                 _at(out), _at(lse), _at(d_out), _at(ws), ws.numel(), _at(g[0]), _at(g[1]), _at(g[2]),
+                                                 _at(g[3]), _hip.stream()), "ocean_attention_bwd")
+        return g[0], g[1], g[2], None, None, None, g[3], None, None, None, None, None
+
+
+def _per_sample(t: torch.Tensor, name: str, B: int, like: torch.Tensor) -> torch.Tensor:
+    _gpu(t, name, like)
+    if t.dtype != torch.int32 or t.shape != (B,):
+        raise ValueError(f"{name} must be an int32 tensor of shape ({B},), got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, mask: Optional[torch.Tensor] = None,
+              key_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
+              query_start: Union[int, torch.Tensor, None] = None, position_table: Optional[torch.Tensor] = None,
+              max_distance: int = 128, bidirectional: bool = True) -> torch.Tensor:
+    """softmax(scale * Q K^T + position bias) V without the weights in memory, for training (the backward pass recomputes
+    them) and serving (single tokens over a long cache); ScaledDotProductAttention (multi_factor_attention.py:34-65) is the form
+    that returns the weights.
+
+    query [batch, heads, queries, d], key / value [batch, key heads, keys, d] in fp32 or bf16, d at most 128, any strides (a
+    transposed view of a projection's [batch, length, heads * d] needs no copy; the result has the query's memory order).
+    Query heads share key heads in equal groups.  Products and sums accumulate in fp32; the probabilities enter the second
+    product in the inputs' type.
+
+    mask: bool or uint8, broadcastable to [batch, heads, queries, keys], nonzero = allowed.  key_lengths: int32 [batch] on the
+    GPU, each sample's key count (clamped to 0..keys); what lies behind is never read, its gradient is zero.  A place that a
+    mask or `causal` takes from some queries only still enters their sums with weight zero, so it has to be finite.  A query
+    with no allowed key gets zeros, and passes no gradient.
+    query_start: position of the first query among the keys, an int or int32 [batch] on the GPU; default keys - queries (the
+    queries are the last keys).  It places `causal` (keys up to the query's own position) and the position bias.
+    position_table [buckets, heads]: the learned bias of the distance key - query position, added to the scaled scores.
+    bidirectional: half of the buckets for each sign; else keys after the query count as distance 0.  With E = half of one
+    side's buckets, distances below E have a bucket each, the others share the rest in logarithmic steps up to max_distance
+    (at most 2048; 128 buckets at most)."""
+    if query.dim() != 4 or key.dim() != 4 or value.shape != key.shape:
+        raise ValueError(f"query [batch, heads, queries, d] and key, value [batch, key heads, keys, d] expected, got {tuple(query.shape)}, "
+                         f"{tuple(key.shape)}, {tuple(value.shape)}")
+    B, H, Lq, d = query.shape
+    Hk, Lk = key.shape[1], key.shape[2]
+    if key.shape[0] != B or key.shape[3] != d or Hk == 0 or H == 0 or H % Hk != 0:
+        raise ValueError(f"key heads must divide the heads, batch and d must agree: query {tuple(query.shape)}, key {tuple(key.shape)}")
+    if query.dtype not in (torch.float32, torch.bfloat16) or key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError(f"attention takes fp32 or bf16 inputs of one type, got {query.dtype}, {key.dtype}, {value.dtype}")
+    if not 1 <= d <= 128:
+        raise ValueError(f"attention takes 1 to 128 features a head, got {d}")
+    _gpu(query, "query")
+    _gpu(key, "key", query)
+    _gpu(value, "value", query)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < 3.0e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if mask is not None:
+        _gpu(mask, "mask", query)
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"mask must be bool or uint8 (nonzero = allowed), got {mask.dtype}")
+        mask = mask.view(torch.uint8).expand(B, H, Lq, Lk)
+    if key_lengths is not None:
+        key_lengths = _per_sample(key_lengths, "key_lengths", B, query)
+    starts, start = None, Lk - Lq
+    if isinstance(query_start, torch.Tensor):
+        starts = _per_sample(query_start, "query_start", B, query)
+    elif query_start is not None:
+        start = int(query_start)
+    if not -(1 << 30) <= start <= (1 << 30):
+        raise ValueError(f"query_start must be within 2^30, got {start}")
+    if position_table is not None:
+        _gpu(position_table, "position_table", query)
+        if position_table.dim() != 2 or position_table.shape[1] != H or not position_table.is_floating_point():
+            raise ValueError(f"position_table must be [buckets, {H}], got {tuple(position_table.shape)} {position_table.dtype}")
+        nb = position_table.shape[0]
+        side = nb // 2 if bidirectional else nb
+        if side < 2 or nb > 128 or (bidirectional and nb % 2):
+            raise ValueError(f"2 to 128 buckets expected (an even number, 4 at least, when bidirectional), got {nb}")
+        if not side // 2 < max_distance <= 2048:
+            raise ValueError(f"max_distance must be above {side // 2} and at most 2048, got {max_distance}")
+        position_table = position_table.float().contiguous()
+    rows = lambda t: t if t.stride(3) == 1 else t.contiguous()
+    least = 4 if query.dtype == torch.float32 else 8
+    if d < least:                                             # the kernels read 16 bytes at a time
+        pad = lambda t: torch.nn.functional.pad(t, (0, least - d))
+        query, key, value = pad(query), pad(key), pad(value)
+    out = _Attention.apply(rows(query), rows(key), rows(value), mask, key_lengths, starts, position_table, int(bool(causal)), start, scale,
+                           int(max_distance), int(bool(bidirectional)))
+    return out[..., :d] if d < least else out
+
+
+def _row_stride(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """`t` (or a dense copy) as rows of its last dimension at one stride."""
+    W = t.shape[-1]
+    rows = t.numel() // W
+    if t.is_contiguous():
+        return t, W
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= W:
+        return t, t.stride(0) if rows > 1 else W
+    return t.contiguous(), W
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        L = _hip.lib()
+        ctx.set_materialize_grads(False)
+        sh = _hip.LayerNormShape()
+        W = x.shape[-1]
+        sh.rows, sh.width, sh.dtype, sh.eps = x.numel() // W, W, _DTYPES[x.dtype], eps
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        total = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if x.numel() == 0:
+            ctx.save_for_backward(x if total is None else total, None, weight)
+        else:
+            train = any(ctx.needs_input_grad)
+            with _on(x.device):
+                xr, sh.x_stride = _row_stride(x)
+                rr = None
+                if residual is not None:
+                    rr, sh.residual_stride = _row_stride(residual)
+                stats = torch.empty(sh.rows, 2, device=x.device, dtype=torch.float32) if train else None
+                _hip.check(L.ocean_layer_norm_fwd(ctypes.byref(sh), _at(xr), _at(rr), _at(weight), _at(bias), _at(y), _at(total), _at(stats),
+                                                  _hip.stream()), "ocean_layer_norm_fwd")
+            if total is not None:
+                sh.x_stride = W
+            if train:
+                ctx.save_for_backward(xr if total is None else total, stats, weight)
+        ctx.sh, ctx.shape = sh, x.shape
+        return y if total is None else (y, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, d_sum=None):
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        if dy is None and d_sum is None:
+            return None, None, None, None, None
+        L = _hip.lib()
+        sh = ctx.sh
+        x, stats, weight = ctx.saved_tensors
+        if dy is None:                                        # only the sum was used
+            zeros = lambda n: torch.zeros(sh.width, device=x.device, dtype=torch.float32) if n else None
+            return d_sum if need_x else None, d_sum if need_r else None, zeros(need_w), zeros(need_b), None
+        dx = torch.empty(ctx.shape, device=x.device, dtype=x.dtype) if need_x or need_r else None
+        dw = torch.empty(sh.width, device=x.device, dtype=torch.float32) if need_w else None
+        db = torch.empty(sh.width, device=x.device, dtype=torch.float32) if need_b else None
+        if x.numel() == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        else:
+            with _on(x.device):
+                dyr, sh.dy_stride = _row_stride(dy)
+                dsr = None
+                if d_sum is not None:
+                    dsr, sh.dsum_stride = _row_stride(d_sum)
+                ws = torch.empty(L.ocean_layer_norm_bwd_workspace(ctypes.byref(sh)), device=x.device, dtype=torch.float32) \
+                    if need_w or need_b else None
+                _hip.check(L.ocean_layer_norm_bwd(ctypes.byref(sh), _at(x), _at(stats), _at(weight), _at(dyr), _at(dsr), _at(ws),
+                                                  0 if ws is None else ws.numel(), _at(dx), _at(dw), _at(db), _hip.stream()),
+                           "ocean_layer_norm_bwd")
+        return dx if need_x else None, dx if need_r else None, dw, db, None
+
+
+def _norm_args(x: torch.Tensor, residual, weight, bias, eps: float):
+    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] > (1 << 24):
+        raise ValueError(f"layer_norm takes [..., width] with 1 to 2^24 columns, got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"layer_norm takes fp32, bf16 or fp16 rows, got {x.dtype}")
+    _gpu(x, "x")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if residual is not None:
+        _gpu(residual, "residual", x)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"x and residual must agree in shape and type, got {tuple(x.shape)} {x.dtype}, {tuple(residual.shape)} {residual.dtype}")
+    out = []
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _gpu(t, name, x)
+            if t.shape != x.shape[-1:] or not t.is_floating_point():
+                raise ValueError(f"{name} must be [{x.shape[-1]}], got {tuple(t.shape)} {t.dtype}")
+            t = t.float().contiguous()
+        out.append(t)
+    return out
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, any width, fp32, bf16 or fp16 (statistics and
+    the weights' gradients in fp32, the latter summed in a fixed order); weight and bias [width] in any floating type, or None."""
+    weight, bias = _norm_args(x, None, weight, bias, eps)
+    return _LayerNorm.apply(x, None, weight, bias, float(eps))
+
+
+def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                   eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(layer_norm(s), s) with s = x + residual, rounded to their type, in one pass; the gradient of s joins the norm's."""
+    weight, bias = _norm_args(x, residual, weight, bias, eps)
+    return _LayerNorm.apply(x, residual, weight, bias, float(eps))
