@@ -575,7 +575,8 @@ int ocean_clip_adam_step_auto(const ocean_adam_chunk* table, int n_chunks, ocean
  * elements for batch, head, position (any; 0 = broadcast for inputs).  mask strides in bytes for b, h, i, j.
  * lse [B, H, Lq] (may be NULL in the forward call): what the backward call needs besides the inputs and `out`.
  * The backward call recomputes the probabilities; dq / dk / dv / dtable are overwritten, each may be NULL (dk / dv rows past a
- * sample's length are zeros); sums run in a fixed order.  Workspaces in floats (0: none needed, or a bad shape). */
+ * sample's length are zeros); sums run in a fixed order.  Workspaces in floats, 16-byte aligned (0: none needed, or a bad
+ * shape); ocean_attention_bwd_workspace reads go_strides too. */
 #define OCEAN_F32 0
 #define OCEAN_BF16 1
 #define OCEAN_F16 2                /* layer norm only */
@@ -588,6 +589,8 @@ typedef struct {
   int num_buckets;                 /* 0: no position bias; at most 128 */
   int max_distance;                /* > E, at most 2048 */
   int bidirectional;
+  int unaligned;                   /* bits 0..3: q, k, v, d_out do not begin on a 16-byte boundary (refused if they do not and the
+                                      bit is missing); such inputs, and those of odd strides or d, are copied to the workspace */
   long q_strides[3], k_strides[3], v_strides[3], o_strides[3];
   long go_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
   long mask_strides[4];

@@ -170,6 +170,29 @@ template <typename T, int D, int ROWS, int THREADS> struct Stage {
   }
 };
 
+// The same tile straight from global memory into LDS, 16 bytes a lane, in flight until wait_tiles(): no registers, no LDS
+// writes.  A wave's 64 lanes fill 1024 consecutive bytes, so the permutation within a row is made on the global side.  Needs
+// 16-byte aligned rows of whole chunks (Params::whole); rows and features past the end come from a line of zeros.
+static __device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
+template <typename T, int D, int ROWS, int THREADS> struct Async {
+  typedef Tile<T, D> TL;
+  static constexpr int kN = ROWS * TL::kCh / THREADS, E = Mm<T>::kEpc;
+  static_assert(ROWS * TL::kCh % THREADS == 0, "a tile is whole rounds of the block");
+  static __device__ __forceinline__ void load(char* t, const T* base, long stride, int row0, int rows, int d, int tid) {
+    char* const to = t + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+    const bool inside = row0 + ROWS <= rows;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int id = tid + n * THREADS, row = id / TL::kCh, c = (id % TL::kCh) ^ TL::swz(row);
+      const T* from = base + (long)(row0 + row) * stride + c * E;
+      if (!(inside || row0 + row < rows) || c * E >= d) from = reinterpret_cast<const T*>(kZeros);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)(to + n * THREADS * 16), 16, 0, 0);
+    }
+  }
+};
+// every load into LDS of this wave has arrived (vmcnt 0; the other counters are left alone)
+__device__ __forceinline__ void wait_tiles() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // a wave's 32 rows as right operand: lane & 31 takes `row` (null: zeros)
 template <typename T, int D> struct RowRegs {
   static constexpr int kSteps = D / (2 * Mm<T>::kEpc);

@@ -5,6 +5,7 @@ namespace {
 
 using seqattn::Params;
 using seqattn::View;
+using seqattn::u32x4;
 
 View view(const void* p, const long* st) { View v; v.p = p; v.b = st[0]; v.h = st[1]; v.l = st[2]; return v; }
 
@@ -21,7 +22,41 @@ void bucket_limits(Params& p) {
   }
 }
 
-struct Plan { int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, parts_at; };
+// The tile loads of the kernels take 16-byte aligned rows of whole 16-byte chunks.  Inputs that are not (odd features or strides)
+// are copied once into the workspace, rows padded with zeros: two passes over an input next to the products over pairs of rows.
+template <typename T> __global__ __launch_bounds__(256) void pack_kernel(const View in, u32x4* __restrict__ out, int heads, int L, int d, int chunks, long n) {
+  for (long x = (long)blockIdx.x * 256 + threadIdx.x; x < n; x += (long)gridDim.x * 256) {
+    const int c = (int)(x % chunks);
+    const long row = x / chunks, bh = row / L;
+    const T* from = (const T*)in.p + bh / heads * in.b + bh % heads * in.h + row % L * in.l;
+    out[x] = seqattn::load_chunk<T>(from, c * seqattn::Mm<T>::kEpc, d);
+  }
+}
+
+bool loose(const ocean_attention_shape* s, const long* st, int bit) {
+  const int E = s->dtype == OCEAN_F32 ? 4 : 8;
+  return (s->unaligned >> bit & 1) || s->d % E || st[0] % E || st[1] % E || st[2] % E;
+}
+size_t packed_floats(const ocean_attention_shape* s, int heads, int L) {
+  const int E = s->dtype == OCEAN_F32 ? 4 : 8;
+  return (size_t)s->B * heads * L * ((s->d + E - 1) / E) * 4;
+}
+// copies `v` to *ws if it has to be (advancing *ws); a base that is less aligned than the caller said is refused
+int pack(const ocean_attention_shape* s, View* v, const long* st, int bit, int heads, int L, float** ws, hipStream_t stream) {
+  if (!loose(s, st, bit)) return reinterpret_cast<uintptr_t>(v->p) % 16 ? OCEAN_ERR_BAD_SHAPE : OCEAN_OK;
+  const int E = s->dtype == OCEAN_F32 ? 4 : 8, chunks = (s->d + E - 1) / E;
+  const long n = (long)s->B * heads * L * chunks;
+  const unsigned blocks = (unsigned)(n < 256L * 4096 ? (n + 255) / 256 : 4096);
+  u32x4* out = reinterpret_cast<u32x4*>(*ws);
+  if (s->dtype == OCEAN_F32) hipLaunchKernelGGL(pack_kernel<float>, dim3(blocks), dim3(256), 0, stream, *v, out, heads, L, s->d, chunks, n);
+  else hipLaunchKernelGGL(pack_kernel<__bf16>, dim3(blocks), dim3(256), 0, stream, *v, out, heads, L, s->d, chunks, n);
+  OCEAN_LAUNCH_CHECK();
+  *v = View{out, (long)heads * L * chunks * E, (long)L * chunks * E, (long)chunks * E};
+  *ws += (size_t)n * 4;
+  return OCEAN_OK;
+}
+
+struct Plan { int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
   if (!s) return OCEAN_ERR_NULL;
@@ -50,8 +85,18 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   pl->splits = (int)(want < 1 ? 1 : want);
   if (base * pl->splits > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;
   pl->fwd_floats = pl->split && pl->splits > 1 ? (size_t)base * pl->splits * 32 * (pl->D + 2) : 0;
+  if (!pl->split) {
+    if (loose(s, s->k_strides, 1)) pl->fwd_floats += packed_floats(s, s->Hk, s->Lk);
+    if (loose(s, s->v_strides, 2)) pl->fwd_floats += packed_floats(s, s->Hk, s->Lk);
+  }
+  size_t at = 0;                                            // backward: packed inputs (the caller's first), delta, sums by bucket
+  if (loose(s, s->q_strides, 0)) at += packed_floats(s, s->H, s->Lq);
+  if (loose(s, s->k_strides, 1)) at += packed_floats(s, s->Hk, s->Lk);
+  if (loose(s, s->v_strides, 2)) at += packed_floats(s, s->Hk, s->Lk);
+  if (loose(s, s->go_strides, 3)) at += packed_floats(s, s->H, s->Lq);
   const size_t rows = (size_t)s->B * s->H * s->Lq;
-  pl->parts_at = (rows + 3) & ~size_t(3);
+  pl->delta_at = at;
+  pl->parts_at = at + ((rows + 3) & ~size_t(3));
   pl->bwd_floats = pl->parts_at + (size_t)s->B * s->H * ((s->Lk + 127) / 128) * (s->num_buckets > 0 ? s->num_buckets : 0);
   return OCEAN_OK;
 }
@@ -91,6 +136,7 @@ int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const voi
   OCEAN_TRY(fill(s, pl, q, k, v, mask, lengths, starts, table, &p));
   if (!out || (pl.fwd_floats && !ws)) return OCEAN_ERR_NULL;
   if (ws_floats < pl.fwd_floats) return OCEAN_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return OCEAN_ERR_BAD_SHAPE;
   p.o = view(out, s->o_strides);
   p.lse = lse;
   if (pl.split) {
@@ -99,6 +145,9 @@ int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const voi
     const size_t rows = (size_t)s->B * s->Hk * pl.chunks * pl.splits * 32;
     p.part_o = ws;
     p.part_ml = ws + rows * pl.D;
+  } else {
+    OCEAN_TRY(pack(s, &p.k, s->k_strides, 1, s->Hk, s->Lk, &ws, (hipStream_t)stream));
+    OCEAN_TRY(pack(s, &p.v, s->v_strides, 2, s->Hk, s->Lk, &ws, (hipStream_t)stream));
   }
   return seqattn::launch_forward(p, s->dtype, (hipStream_t)stream);
 }
@@ -114,8 +163,13 @@ int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const voi
   if (ws_floats < pl.bwd_floats) return OCEAN_ERR_WORKSPACE;
   p.o = view(out, s->o_strides); p.go = view(d_out, s->go_strides); p.lse = const_cast<float*>(lse);
   p.dq = view(dq, s->dq_strides); p.dk = view(dk, s->dk_strides); p.dv = view(dv, s->dv_strides);
-  p.delta = ws;
+  p.delta = ws + pl.delta_at;
   p.dtable_part = dtable ? ws + pl.parts_at : nullptr;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return OCEAN_ERR_BAD_SHAPE;
+  OCEAN_TRY(pack(s, &p.q, s->q_strides, 0, s->H, s->Lq, &ws, (hipStream_t)stream));
+  OCEAN_TRY(pack(s, &p.k, s->k_strides, 1, s->Hk, s->Lk, &ws, (hipStream_t)stream));
+  OCEAN_TRY(pack(s, &p.v, s->v_strides, 2, s->Hk, s->Lk, &ws, (hipStream_t)stream));
+  OCEAN_TRY(pack(s, &p.go, s->go_strides, 3, s->H, s->Lq, &ws, (hipStream_t)stream));
   return seqattn::launch_backward(p, s->dtype, dtable, (hipStream_t)stream);
 }
 

@@ -12,7 +12,7 @@ namespace {
 constexpr int kRows = 128;           // queries (keys) of a block: four waves, 32 each
 
 // p_ij for keys j0.. of this lane's query, from scores
-template <bool BIAS> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int keys,
+template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int keys,
                                                                    const uint8_t* mrow, const float* lut, bool edge, int lane) {
   const int h4 = 4 * (lane >> 5);
 #pragma unroll
@@ -20,14 +20,14 @@ template <bool BIAS> __device__ __forceinline__ void probabilities(const Params&
     const float t = BIAS ? lut[dist_slot(p, j0 + 8 * (r >> 2) + h4 + (r & 3) - pos)] - lse : -lse;
     s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
   }
-  if (edge) {
-    const int end = p.causal ? min(keys, pos + 1) : keys;
+  if (MASK || edge) {
+    const int end = (p.causal ? min(keys, pos + 1) : keys) - j0 - h4;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int j = j0 + 8 * g + h4;
-      const uint32_t ok = mrow ? mask4(p, mrow, j, keys) : 15u;
+      uint32_t ok = 15u;
+      if (MASK) ok = mrow ? mask4(p, mrow, j0 + 8 * g + h4, keys) : 15u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (j + e >= end || !((ok >> e) & 1u)) s[4 * g + e] = 0.f;
+      for (int e = 0; e < 4; ++e) if (8 * g + e >= end || (MASK && !((ok >> e) & 1u))) s[4 * g + e] = 0.f;
     }
   }
 }
@@ -96,7 +96,7 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
 
 template <typename T, int D> struct BwdTile { static constexpr int kRows = sizeof(T) == 2 ? 64 : 32; };
 
-template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void dq_kernel(const Params p) {
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BN = BwdTile<T, D>::kRows, NS = BN / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -128,7 +128,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
   }
   delta = other_half_sum(delta);
   float rest = 0.f;
-  const uint8_t* mrow = p.mask && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
+  const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
   int end = keys, wend = keys, wfull = keys;
   if (p.causal) {
     end = min(end, start + min(tile * kRows + kRows, p.Lq));
@@ -139,31 +139,28 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
   f32x16 acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
-  Stage<T, D, BN, 256> ks, vs;
+  typedef Async<T, D, BN, 256> Load;
   const int tiles = end > 0 ? (end + BN - 1) / BN : 0;
   if (tiles > 0) {
-    ks.fetch(kb, p.k.l, 0, keys, p.d, tid);
-    vs.fetch(vb, p.v.l, 0, keys, p.d, tid);
-    ks.put(kt, tid);
-    vs.put(vt, tid);
+    Load::load(kt, kb, p.k.l, 0, keys, p.d, tid);
+    Load::load(vt, vb, p.v.l, 0, keys, p.d, tid);
   }
   // Up to two tiles of keys sit in the two buffers.  Rows of so few keys are where 16-bit rounding of `o` reaches dq through delta
   // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first.
   const bool few = sizeof(T) == 2 && tiles <= 2;
   if (few && tiles == 2) {
-    ks.fetch(kb, p.k.l, BN, keys, p.d, tid);
-    vs.fetch(vb, p.v.l, BN, keys, p.d, tid);
-    ks.put(kt + kBuf, tid);
-    vs.put(vt + kBuf, tid);
+    Load::load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid);
+    Load::load(vt + kBuf, vb, p.v.l, BN, keys, p.d, tid);
   }
-  __syncthreads();
   if (few) {
+    wait_tiles();
+    __syncthreads();
     float sum = 0.f;
     for (int j = 0; j < wend; j += 32) {
       const int at = j / BN * kBuf, row = j % BN;
       f32x16 s = row_mma<T, D>(kt + at, row, lane, q, f32x16{});
       const f32x16 dp = row_mma<T, D>(vt + at, row, lane, go, f32x16{});
-      probabilities<BIAS>(p, s, c, lse, j, pos, keys, mrow, lut, p.mask || j + 32 > wfull, lane);
+      probabilities<BIAS, MASK>(p, s, c, lse, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum = fmaf(s[r], dp[r], sum);
     }
@@ -171,10 +168,13 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
   }
   for (int t = 0; t < tiles; ++t) {
     const int j0 = t * BN, cur = t & 1;
-    const bool more = t + 1 < tiles && !few;
-    if (more) {
-      ks.fetch(kb, p.k.l, j0 + BN, keys, p.d, tid);
-      vs.fetch(vb, p.v.l, j0 + BN, keys, p.d, tid);
+    if (!few) {
+      wait_tiles();
+      __syncthreads();
+      if (t + 1 < tiles) {
+        Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
+        Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
+      }
     }
     if (j0 < wend) {
 #pragma unroll
@@ -182,7 +182,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
         const int j = j0 + 32 * n;
         f32x16 s = row_mma<T, D>(kt + cur * kBuf, 32 * n, lane, q, f32x16{});
         const f32x16 dp = row_mma<T, D>(vt + cur * kBuf, 32 * n, lane, go, f32x16{});
-        probabilities<BIAS>(p, s, c, lse, j, pos, keys, mrow, lut, p.mask || j + 32 > wfull, lane);
+        probabilities<BIAS, MASK>(p, s, c, lse, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] *= dp[r] - delta;
@@ -194,11 +194,6 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
         for (int db = 0; db < D / 32; ++db) acc[db] = col_mma<D>(kt + cur * kBuf, 32 * n, db, lane, pf, acc[db]);
       }
     }
-    if (more) {
-      ks.put(kt + (cur ^ 1) * kBuf, tid);
-      vs.put(vt + (cur ^ 1) * kBuf, tid);
-    }
-    __syncthreads();
   }
   if (live && p.dq.p) store_row<T, D>((T*)p.dq.p + b * p.dq.b + head * p.dq.h + (long)i * p.dq.l, acc, p.scale, p.d, lane);
   // In 16 bits `o` was rounded, and so were the weights that formed it: delta is a few 1e-3 of |do| |o| off.  The row's ds sum to
@@ -207,7 +202,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
   if (live && lane < 32) p.delta[((long)b * p.H + head) * p.Lq + i] = delta;
 }
 
-template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void dkv_kernel(const Params p, const int k_tiles) {
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Params p, const int k_tiles) {
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -248,34 +243,32 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
   if (tile * kRows >= keys) first = p.Lq;
   const int t0 = first / BM, tiles = (p.Lq + BM - 1) / BM - t0, all = tiles * p.G;
   const int head0 = kh * p.G;
-  Stage<T, D, BM, 256> qs, gs;
+  typedef Async<T, D, BM, 256> Load;
   float rv = 0.f;                                           // threads 0..BM-1: lse, BM..2BM-1: delta
-  const auto fetch = [&](int u) {
+  const auto load = [&](int u, int buf) {
     const int head = head0 + u / tiles, r0 = (t0 + u % tiles) * BM;
-    qs.fetch((const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
-    gs.fetch((const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
     if (tid < 2 * BM) {
       const int i = r0 + tid % BM;
-      const bool in = i < p.Lq;
       const float* from = tid < BM ? p.lse : p.delta;
-      rv = in ? from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? INFINITY : 0.f;
+      rv = i < p.Lq ? from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? INFINITY : 0.f;
     }
+    Load::load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
+    Load::load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
   };
-  const auto put = [&](int cur) {
-    qs.put(qt + cur * kBuf, tid);
-    gs.put(gt + cur * kBuf, tid);
-    if (tid < 2 * BM) rowv[cur * 2 * BM + tid] = rv;
-  };
-  if (all > 0) { fetch(0); put(0); }
-  if (BIAS && all > 0) fill_bias(p, head0, lut, tid, 256);
-  __syncthreads();
+  if (all > 0) {
+    load(0, 0);
+    if (BIAS) fill_bias(p, head0, lut, tid, 256);
+  }
   for (int u = 0; u < all; ++u) {
     const int cur = u & 1, g = u / tiles, head = head0 + g, r0 = (t0 + u % tiles) * BM;
+    if (tid < 2 * BM) rowv[cur * 2 * BM + tid] = rv;
     if (BIAS && u > 0 && u % tiles == 0) {
+      __syncthreads();                                      // the last head's biases are still being read
       fill_bias(p, head, lut, tid, 256);
-      __syncthreads();
     }
-    if (u + 1 < all) fetch(u + 1);
+    wait_tiles();
+    __syncthreads();
+    if (u + 1 < all) load(u + 1, cur ^ 1);
     if (j0 < keys && r0 + BM > wfirst) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
@@ -289,13 +282,14 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
           const float t = BIAS ? lut[dist_slot(p, j - (start + i0 + h4 + at))] - lr[at] : -lr[at];
           s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
         }
-        if (p.mask || j0 + 32 > keys || (p.causal && i0 < wfull)) {
-          const uint8_t* mcol = p.mask ? p.mask + b * p.mb + head * p.mh + (long)j * p.mj : nullptr;
+        if (MASK || j0 + 32 > keys || (p.causal && i0 < wfull)) {
+          const uint8_t* mcol = MASK ? p.mask + b * p.mb + head * p.mh + (long)j * p.mj + (long)(i0 + h4) * p.mi : nullptr;
+          const int from = live ? (p.causal ? j - start : 0) - i0 - h4 : 1 << 30;      // the first query that sees this key
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int i = i0 + h4 + 8 * (r >> 2) + (r & 3);
-            bool ok = live && !(p.causal && j > start + i);
-            if (mcol && ok && i < p.Lq) ok = mcol[(long)i * p.mi] != 0;
+            const int i = 8 * (r >> 2) + (r & 3);
+            bool ok = i >= from;
+            if (MASK && ok && i0 + h4 + i < p.Lq) ok = mcol[(long)i * p.mi] != 0;
             if (!ok) s[r] = 0.f;
           }
         }
@@ -311,8 +305,6 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void d
         for (int db = 0; db < D / 32; ++db) dk[db] = col_mma<D>(qt + cur * kBuf, 32 * n, db, lane, pf, dk[db]);
       }
     }
-    if (u + 1 < all) put(cur ^ 1);
-    __syncthreads();
     if (sum_bias && u % tiles == tiles - 1) store_bias_sums(p, diag, dist_sums, p.dtable_part + (((long)head * p.B + b) * k_tiles + tile) * p.buckets, tid);
   }
   if (sum_bias && all == 0)
@@ -344,21 +336,21 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
 }
 
-template <typename T, int D, bool BIAS> int backward(const Params& p, float* dtable, hipStream_t s) {
+template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p, float* dtable, hipStream_t s) {
   typedef Tile<T, D> TL;
   constexpr int BN = BwdTile<T, D>::kRows;
   const size_t slots = 2 * p.max_dist + 1;
   size_t lds = 4 * BN * TL::kRowBytes;
   if (BIAS) lds += slots * sizeof(float);
-  OCEAN_TRY(set_lds(dq_kernel<T, D, BIAS>, lds));
-  hipLaunchKernelGGL((dq_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
+  OCEAN_TRY(set_lds(dq_kernel<T, D, BIAS, MASK>, lds));
+  hipLaunchKernelGGL((dq_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
   const int k_tiles = (p.Lk + kRows - 1) / kRows;
   if (p.dk.p || p.dv.p || p.dtable_part) {
     lds = 4 * BN * TL::kRowBytes + 4 * BN * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
     if (BIAS && p.dtable_part) lds += (4 * slots + 4 * 32 * 33) * sizeof(float);
-    OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS>, lds));
-    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.Hk * k_tiles)), dim3(256), lds, s, p, k_tiles);
+    OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS, MASK>, lds));
+    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.Hk * k_tiles)), dim3(256), lds, s, p, k_tiles);
     OCEAN_LAUNCH_CHECK();
   }
   if (BIAS && p.dtable_part) {
@@ -369,7 +361,8 @@ template <typename T, int D, bool BIAS> int backward(const Params& p, float* dta
 }
 
 template <typename T, int D> int backward_b(const Params& p, float* dtable, hipStream_t s) {
-  return p.table ? backward<T, D, true>(p, dtable, s) : backward<T, D, false>(p, dtable, s);
+  if (p.mask) return p.table ? backward<T, D, true, true>(p, dtable, s) : backward<T, D, false, true>(p, dtable, s);
+  return p.table ? backward<T, D, true, false>(p, dtable, s) : backward<T, D, false, false>(p, dtable, s);
 }
 template <typename T> int backward_d(const Params& p, float* dtable, hipStream_t s) {
   if (p.d <= 32) return backward_b<T, 32>(p, dtable, s);

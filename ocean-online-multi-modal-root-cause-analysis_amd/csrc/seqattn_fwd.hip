@@ -39,28 +39,28 @@ template <int N> __device__ __forceinline__ float softmax_step(f32x16 (&s)[N], f
 }
 
 // adds the bias and takes out the places that are not allowed, for keys j0..j0+31 and this lane's query
-template <bool BIAS> __device__ __forceinline__ void adjust(const Params& p, f32x16& s, float mult, int j0, int pos, int keys, const uint8_t* mrow,
+template <bool BIAS, bool MASK> __device__ __forceinline__ void adjust(const Params& p, f32x16& s, float mult, int j0, int pos, int keys, const uint8_t* mrow,
                                                              const float* lut, bool edge, int lane) {
   const int h4 = 4 * (lane >> 5);
   if (BIAS) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mult, lut[dist_slot(p, j0 + 8 * (r >> 2) + h4 + (r & 3) - pos)]);
   }
-  if (edge) {
-    const int end = p.causal ? min(keys, pos + 1) : keys;
+  if (MASK || edge) {
+    const int end = (p.causal ? min(keys, pos + 1) : keys) - j0 - h4;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int j = j0 + 8 * g + h4;
-      const uint32_t ok = mrow ? mask4(p, mrow, j, keys) : 15u;
+      uint32_t ok = 15u;
+      if (MASK) ok = mrow ? mask4(p, mrow, j0 + 8 * g + h4, keys) : 15u;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) if (j + e >= end || !((ok >> e) & 1u)) s[4 * g + e] = -INFINITY;
+      for (int e = 0; e < 4; ++e) if (8 * g + e >= end || (MASK && !((ok >> e) & 1u))) s[4 * g + e] = -INFINITY;
     }
   }
 }
 
 template <typename T, int D> struct FwdTile { static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32; };
 
-template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void fwd_rows_kernel(const Params p) {
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void fwd_rows_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BN = FwdTile<T, D>::kKeys, NS = BN / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -79,7 +79,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
   const bool live = i < p.Lq;
   RowRegs<T, D> q;
   q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
-  const uint8_t* mrow = p.mask && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
+  const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
   int end = keys;                                           // keys that some query of the block may see
   if (p.causal) end = min(end, start + min(tile * kRows + kRows, p.Lq));
   int wend = keys;                                          // .. of this wave; below wfull no place of the wave is behind the diagonal
@@ -91,20 +91,19 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
   f32x16 acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
-  Stage<T, D, BN, 256> ks, vs;
+  typedef Async<T, D, BN, 256> Load;
   const int tiles = end > 0 ? (end + BN - 1) / BN : 0;
   if (tiles > 0) {
-    ks.fetch(kb, p.k.l, 0, keys, p.d, tid);
-    vs.fetch(vb, p.v.l, 0, keys, p.d, tid);
-    ks.put(kt, tid);
-    vs.put(vt, tid);
+    Load::load(kt, kb, p.k.l, 0, keys, p.d, tid);
+    Load::load(vt, vb, p.v.l, 0, keys, p.d, tid);
   }
-  __syncthreads();
   for (int t = 0; t < tiles; ++t) {
     const int j0 = t * BN, cur = t & 1;
+    wait_tiles();
+    __syncthreads();
     if (t + 1 < tiles) {
-      ks.fetch(kb, p.k.l, j0 + BN, keys, p.d, tid);
-      vs.fetch(vb, p.v.l, j0 + BN, keys, p.d, tid);
+      Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
+      Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
     }
     if (j0 < wend) {
       f32x16 s[NS];
@@ -112,7 +111,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
       for (int n = 0; n < NS; ++n) {
         s[n] = row_mma<T, D>(kt + cur * kBuf, 32 * n, lane, q, f32x16{});
         const int j = j0 + 32 * n;
-        adjust<BIAS>(p, s[n], c, j, pos, keys, mrow, lut, p.mask || j + 32 > wfull, lane);
+        adjust<BIAS, MASK>(p, s[n], c, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
       }
       const float f = softmax_step<NS>(s, mult, st);
       if (__any(f != 1.f)) {
@@ -127,11 +126,6 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
         for (int db = 0; db < D / 32; ++db) acc[db] = col_mma<D>(vt + cur * kBuf, 32 * n, db, lane, pf, acc[db]);
       }
     }
-    if (t + 1 < tiles) {
-      ks.put(kt + (cur ^ 1) * kBuf, tid);
-      vs.put(vt + (cur ^ 1) * kBuf, tid);
-    }
-    __syncthreads();
   }
   if (live) {
     const float l = other_half_sum(st.l);
@@ -144,7 +138,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
 // A block's 32 rows are (query, head of the group) pairs of one key head, so a single token's G heads read the keys once; its
 // four waves take 32-key tiles in turn, each through LDS of its own, and the blocks of one row chunk split the keys further.
 // Bound by reading the keys and values once.
-template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void fwd_split_kernel(const Params p) {
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256) void fwd_split_kernel(const Params p) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -164,7 +158,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
   const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
   RowRegs<T, D> q;
   q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
-  const uint8_t* mrow = p.mask && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
+  const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
   const int last = start + min((chunk * 32 + 31) / p.G, p.Lq - 1);
   const int end = p.causal ? min(keys, last + 1) : keys;
   const int full = p.causal ? min(keys, start + chunk * 32 / p.G + 1) : keys;
@@ -200,7 +194,7 @@ template <typename T, int D, bool BIAS> __global__ __launch_bounds__(256) void f
         s[0][r] = fmaf(s[0][r], c, p.table[(long)bmap[dist_slot(p, dist)] * p.H + min(head, p.H - 1)] * kLog2e);
       }
     }
-    adjust<false>(p, s[0], c, j0, pos, keys, mrow, nullptr, p.mask || j0 + 32 > full, lane);
+    adjust<false, MASK>(p, s[0], c, j0, pos, keys, mrow, nullptr, j0 + 32 > full, lane);
     const float f = softmax_step<1>(s, mult, st);
     if (__any(f != 1.f)) {
 #pragma unroll
@@ -293,20 +287,20 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
 }
 
-template <typename T, int D, bool BIAS> int forward(const Params& p, hipStream_t s) {
+template <typename T, int D, bool BIAS, bool MASK> int forward(const Params& p, hipStream_t s) {
   typedef Tile<T, D> TL;
   if (p.splits == 0) {
     const size_t lds = 4 * FwdTile<T, D>::kKeys * TL::kRowBytes + (BIAS ? (2 * p.max_dist + 1) * sizeof(float) : 0);
-    OCEAN_TRY(set_lds(fwd_rows_kernel<T, D, BIAS>, lds));
-    hipLaunchKernelGGL((fwd_rows_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
+    OCEAN_TRY(set_lds(fwd_rows_kernel<T, D, BIAS, MASK>, lds));
+    hipLaunchKernelGGL((fwd_rows_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
     OCEAN_LAUNCH_CHECK();
     return OCEAN_OK;
   }
   size_t lds = 8 * 32 * TL::kRowBytes + (BIAS ? 2 * p.max_dist + 1 : 0);
   const size_t meet = (size_t)(4 * D * 32 + 4 * 2 * 32) * sizeof(float);
   if (meet > lds) lds = meet;
-  OCEAN_TRY(set_lds(fwd_split_kernel<T, D, BIAS>, lds));
-  hipLaunchKernelGGL((fwd_split_kernel<T, D, BIAS>), dim3((unsigned)((long)p.B * p.Hk * p.q_tiles * p.splits)), dim3(256), lds, s, p);
+  OCEAN_TRY(set_lds(fwd_split_kernel<T, D, BIAS, MASK>, lds));
+  hipLaunchKernelGGL((fwd_split_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.Hk * p.q_tiles * p.splits)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
   if (p.splits > 1) {
     hipLaunchKernelGGL((fwd_join_kernel<T, D>), dim3((unsigned)(((long)p.B * p.H * p.Lq + 3) / 4)), dim3(256), 0, s, p);
@@ -315,7 +309,10 @@ template <typename T, int D, bool BIAS> int forward(const Params& p, hipStream_t
   return OCEAN_OK;
 }
 
-template <typename T, int D> int forward_b(const Params& p, hipStream_t s) { return p.table ? forward<T, D, true>(p, s) : forward<T, D, false>(p, s); }
+template <typename T, int D> int forward_b(const Params& p, hipStream_t s) {
+  if (p.mask) return p.table ? forward<T, D, true, true>(p, s) : forward<T, D, false, true>(p, s);
+  return p.table ? forward<T, D, true, false>(p, s) : forward<T, D, false, false>(p, s);
+}
 template <typename T> int forward_d(const Params& p, hipStream_t s) {
   if (p.d <= 32) return forward_b<T, 32>(p, s);
   if (p.d <= 64) return forward_b<T, 64>(p, s);

@@ -125,7 +125,7 @@ class GatConvShape(ctypes.Structure):
 class AttentionShape(ctypes.Structure):
     _fields_ = [("B", c_int), ("H", c_int), ("Hk", c_int), ("Lq", c_int), ("Lk", c_int), ("d", c_int), ("dtype", c_int),
                 ("causal", c_int), ("query_start", c_int), ("scale", c_float), ("num_buckets", c_int), ("max_distance", c_int),
-                ("bidirectional", c_int)] + [(n + "_strides", c_long * 3) for n in ("q", "k", "v", "o", "go", "dq", "dk", "dv")] + [
+                ("bidirectional", c_int), ("unaligned", c_int)] + [(n + "_strides", c_long * 3) for n in ("q", "k", "v", "o", "go", "dq", "dk", "dv")] + [
                 ("mask_strides", c_long * 4)]
 
 

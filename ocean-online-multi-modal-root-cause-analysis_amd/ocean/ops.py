@@ -427,6 +427,7 @@ class _Attention(torch.autograd.Function):
             sh.num_buckets, sh.max_distance, sh.bidirectional = table.shape[0], max_distance, both
         out = _like(q)
         _set_strides(sh.o_strides, out)
+        sh.unaligned = (q.data_ptr() % 16 != 0) | (k.data_ptr() % 16 != 0) << 1 | (v.data_ptr() % 16 != 0) << 2
         ctx.sh = sh
         if q.numel() == 0 or k.numel() == 0:
             ctx.save_for_backward(q, k, v, table)
@@ -456,6 +457,7 @@ class _Attention(torch.autograd.Function):
                 d_out = d_out.contiguous()
             g = [_like(t) if n else None for n, t in zip(need, (q, k, v, table))]
             _set_strides(sh.go_strides, d_out)
+            sh.unaligned = sh.unaligned & 7 | (d_out.data_ptr() % 16 != 0) << 3
             for field, t in zip((sh.dq_strides, sh.dk_strides, sh.dv_strides), g):
                 if t is not None:
                     _set_strides(field, t)
