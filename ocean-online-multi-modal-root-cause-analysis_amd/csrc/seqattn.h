@@ -42,8 +42,9 @@ struct Params {
   const float* table;                // [buckets, H] or null
   int buckets, side, exact, both, max_dist;      // side: buckets of one side; exact: of them, one per distance
   int limits[kMaxBuckets];           // distances where the far buckets exact+1, exact+2, .. begin
-  float* dtable_part;                // [H][B][key tiles][buckets]
-  int splits; float* part_o; float* part_ml;     // forward over split keys: [row chunk][split][rows][..]
+  float* dtable_part;                // [H][B][key tiles][segments][buckets]
+  int k_tiles, segs, seg_tiles;      // launch over keys: tiles of 128 keys, segments of their queries, query tiles (of all heads) a segment
+  int splits; float* part_o; float* part_ml;     // partial results of split sums
   int q_tiles;
 };
 
@@ -288,6 +289,9 @@ __device__ __forceinline__ int die_order(int id, int n) {
   const int per = n >> 3, rem = n & 7, die = id & 7, k = id >> 3;
   return die * per + min(die, rem) + k;
 }
+
+constexpr int kKeyTile = 128;        // keys of a block of the launch over keys
+constexpr int query_tile(bool bits16) { return bits16 ? 64 : 32; }       // and the queries it takes at a time
 
 int launch_forward(const Params& p, int type, hipStream_t s);
 int launch_backward(const Params& p, int type, float* dtable, hipStream_t s);

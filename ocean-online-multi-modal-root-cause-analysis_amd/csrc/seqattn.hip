@@ -56,7 +56,30 @@ int pack(const ocean_attention_shape* s, View* v, const long* st, int bit, int h
   return OCEAN_OK;
 }
 
-struct Plan { int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
+// How many segments the queries of a key tile are split into.  One block holds a key tile's gradients in registers, so with few
+// key tiles, or with `causal` (where the first tile has all queries and the last ones next to none), the chip waits for the longest
+// block.  Segments cost a round trip of fp32 partial sums.  The estimate counts both, in microseconds, from what one query tile
+// and the partial sums were measured to take.
+void plan_segments(const ocean_attention_shape* s, int D, int* segs, int* seg_tiles) {
+  const bool b16 = s->dtype != OCEAN_F32;
+  const int rows = seqattn::query_tile(b16);
+  const long units = (long)s->B * s->Hk * ((s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile);
+  const long tiles = (long)(s->H / s->Hk) * ((s->Lq + rows - 1) / rows);
+  const double slots = D * (b16 ? 2 : 4) > 128 ? 256.0 : 512.0;
+  const double tile_us = (b16 ? 2.5 : 8.0) * D / 128.0 * (slots / 256.0);
+  double best = 1e30;
+  *segs = 1;
+  for (int n = 1; n <= 16 && (n == 1 || n <= tiles / 2); ++n) {
+    const long per = (tiles + n - 1) / n;
+    double load = s->causal ? 0.5 * units * tiles / slots : ceil(units * n / slots) * per;
+    if (s->causal) load = load + 0.25 * per > per ? load + 0.25 * per : per;
+    const double us = load * tile_us + (n > 1 ? 5.0 + (double)units * n * seqattn::kKeyTile * D * 16.0 / 4.0e6 : 0.0);
+    if (us < best) { best = us; *segs = n; }
+  }
+  *seg_tiles = (int)((tiles + *segs - 1) / *segs);
+}
+
+struct Plan { int segs, seg_tiles; size_t part_at; int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
   if (!s) return OCEAN_ERR_NULL;
@@ -74,7 +97,7 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   }
   pl->D = (s->d + 31) / 32 * 32;
   const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
-  if (blocks > 0x7fffffffL || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffffL || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL / 16) return OCEAN_ERR_UNSUPPORTED;
   // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as rows.
   pl->split = (long)s->Lq * G <= 32;
   pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
@@ -97,7 +120,10 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const size_t rows = (size_t)s->B * s->H * s->Lq;
   pl->delta_at = at;
   pl->parts_at = at + ((rows + 3) & ~size_t(3));
-  pl->bwd_floats = pl->parts_at + (size_t)s->B * s->H * ((s->Lk + 127) / 128) * (s->num_buckets > 0 ? s->num_buckets : 0);
+  plan_segments(s, pl->D, &pl->segs, &pl->seg_tiles);
+  const size_t k_tiles = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;
+  pl->part_at = pl->parts_at + (((size_t)s->B * s->H * k_tiles * pl->segs * (s->num_buckets > 0 ? s->num_buckets : 0) + 3) & ~size_t(3));
+  pl->bwd_floats = pl->part_at + (pl->segs > 1 ? (size_t)s->B * s->Hk * k_tiles * pl->segs * seqattn::kKeyTile * pl->D * 2 : 0);
   return OCEAN_OK;
 }
 
@@ -165,6 +191,10 @@ int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const voi
   p.dq = view(dq, s->dq_strides); p.dk = view(dk, s->dk_strides); p.dv = view(dv, s->dv_strides);
   p.delta = ws + pl.delta_at;
   p.dtable_part = dtable ? ws + pl.parts_at : nullptr;
+  p.part_o = ws + pl.part_at;
+  p.k_tiles = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;
+  p.segs = pl.segs;
+  p.seg_tiles = pl.seg_tiles;
   if (reinterpret_cast<uintptr_t>(ws) % 16) return OCEAN_ERR_BAD_SHAPE;
   OCEAN_TRY(pack(s, &p.q, s->q_strides, 0, s->H, s->Lq, &ws, (hipStream_t)stream));
   OCEAN_TRY(pack(s, &p.k, s->k_strides, 1, s->Hk, s->Lk, &ws, (hipStream_t)stream));

@@ -9,7 +9,7 @@
 namespace seqattn {
 namespace {
 
-constexpr int kRows = 128;           // queries (keys) of a block: four waves, 32 each
+constexpr int kRows = kKeyTile;      // queries (keys) of a block: four waves, 32 each
 
 // p_ij for keys j0.. of this lane's query, from scores
 template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int keys,
@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
   __syncthreads();
 }
 
-template <typename T, int D> struct BwdTile { static constexpr int kRows = sizeof(T) == 2 ? 64 : 32; };
+template <typename T, int D> struct BwdTile { static constexpr int kRows = query_tile(sizeof(T) == 2); };
 
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
@@ -202,7 +202,15 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   if (live && lane < 32) p.delta[((long)b * p.H + head) * p.Lq + i] = delta;
 }
 
-template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Params p, const int k_tiles) {
+// the tiles of BM queries that see some key of the tile: `tiles` from t0 on
+template <int BM> __device__ __forceinline__ void query_tiles(const Params& p, int tile, int keys, int start, int* t0, int* tiles) {
+  int first = p.causal ? min(max(tile * kRows - start, 0), p.Lq) : 0;
+  if (tile * kRows >= keys) first = p.Lq;
+  *t0 = first / BM;
+  *tiles = first < p.Lq ? (p.Lq + BM - 1) / BM - *t0 : 0;
+}
+
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -221,8 +229,10 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     diag.below = diag.above = 0.f;
     if (sum_bias) for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
   }
-  const int id = die_order(blockIdx.x, gridDim.x);
-  const int tile = id % k_tiles, bk = id / k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
+  // Work list: key head by key head; for each, the first segment of every key tile, then the second, ..  With `causal` the first
+  // tiles have the most queries, so the large pieces start first and the small ones fill the gaps.
+  const int k_tiles = p.k_tiles, id = die_order(blockIdx.x, gridDim.x);
+  const int tile = id % k_tiles, seg = id / k_tiles % p.segs, bk = id / (k_tiles * p.segs), b = bk / p.Hk, kh = bk % p.Hk;
   const int keys = keys_of(p, b), start = start_of(p, b);
   const int j0 = tile * kRows + 32 * w, j = j0 + (lane & 31);
   const bool live = j < keys;
@@ -233,15 +243,12 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) { dk[db] = f32x16{}; dv[db] = f32x16{}; }
-  // queries from `first` on see some key of the block (of this wave); from `full` on all keys of this wave
-  int first = 0, wfirst = 0, wfull = 0;
-  if (p.causal) {
-    first = min(max(tile * kRows - start, 0), p.Lq);
-    wfirst = max(j0 - start, 0);
-    wfull = j0 + 31 - start;
-  }
-  if (tile * kRows >= keys) first = p.Lq;
-  const int t0 = first / BM, tiles = (p.Lq + BM - 1) / BM - t0, all = tiles * p.G;
+  // queries from wfirst on see some key of this wave; from wfull on every key
+  int wfirst = 0, wfull = 0;
+  if (p.causal) { wfirst = max(j0 - start, 0); wfull = j0 + 31 - start; }
+  int t0, tiles;
+  query_tiles<BM>(p, tile, keys, start, &t0, &tiles);
+  const int all = tiles * p.G, u0 = min(seg * p.seg_tiles, all), u1 = min(u0 + p.seg_tiles, all);
   const int head0 = kh * p.G;
   typedef Async<T, D, BM, 256> Load;
   float rv = 0.f;                                           // threads 0..BM-1: lse, BM..2BM-1: delta
@@ -255,20 +262,20 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     Load::load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
     Load::load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
   };
-  if (all > 0) {
-    load(0, 0);
-    if (BIAS) fill_bias(p, head0, lut, tid, 256);
+  if (u0 < u1) {
+    load(u0, u0 & 1);
+    if (BIAS) fill_bias(p, head0 + u0 / tiles, lut, tid, 256);
   }
-  for (int u = 0; u < all; ++u) {
+  for (int u = u0; u < u1; ++u) {
     const int cur = u & 1, g = u / tiles, head = head0 + g, r0 = (t0 + u % tiles) * BM;
     if (tid < 2 * BM) rowv[cur * 2 * BM + tid] = rv;
-    if (BIAS && u > 0 && u % tiles == 0) {
+    if (BIAS && u > u0 && u % tiles == 0) {
       __syncthreads();                                      // the last head's biases are still being read
       fill_bias(p, head, lut, tid, 256);
     }
     wait_tiles();
     __syncthreads();
-    if (u + 1 < all) load(u + 1, cur ^ 1);
+    if (u + 1 < u1) load(u + 1, cur ^ 1);
     if (j0 < keys && r0 + BM > wfirst) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
@@ -305,13 +312,53 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         for (int db = 0; db < D / 32; ++db) dk[db] = col_mma<D>(qt + cur * kBuf, 32 * n, db, lane, pf, dk[db]);
       }
     }
-    if (sum_bias && u % tiles == tiles - 1) store_bias_sums(p, diag, dist_sums, p.dtable_part + (((long)head * p.B + b) * k_tiles + tile) * p.buckets, tid);
+    if (sum_bias && (u == u1 - 1 || u % tiles == tiles - 1))
+      store_bias_sums(p, diag, dist_sums, p.dtable_part + ((((long)head * p.B + b) * k_tiles + tile) * p.segs + seg) * p.buckets, tid);
   }
-  if (sum_bias && all == 0)
-    for (int x = tid; x < p.G * p.buckets; x += 256) p.dtable_part[(((long)(head0 + x / p.buckets) * p.B + b) * k_tiles + tile) * p.buckets + x % p.buckets] = 0.f;
+  if (sum_bias) {                                           // the heads that this segment does not reach
+    const int g0 = u0 < u1 ? u0 / tiles : 0, g1 = u0 < u1 ? (u1 - 1) / tiles : -1;
+    for (int x = tid; x < p.G * p.buckets; x += 256) {
+      const int g = x / p.buckets;
+      if (g < g0 || g > g1) p.dtable_part[((((long)(head0 + g) * p.B + b) * k_tiles + tile) * p.segs + seg) * p.buckets + x % p.buckets] = 0.f;
+    }
+  }
+  if (seg > 0 && u0 >= u1) return;
+  if (all > p.seg_tiles) {                                  // more than one segment: sums in the matrix instructions' layout
+    float* part = p.part_o + ((((long)bk * k_tiles + tile) * p.segs + seg) * 4 + w) * (2 * 32 * D) + lane * 4;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        *reinterpret_cast<f32x4*>(part + (db * 4 + g) * 256) = f32x4{dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(part + 32 * D + (db * 4 + g) * 256) = f32x4{dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]};
+      }
+    return;
+  }
   if (j < p.Lk) {                                           // keys past the sample's end get zeros
     if (p.dk.p) store_row<T, D>((T*)p.dk.p + b * p.dk.b + kh * p.dk.h + (long)j * p.dk.l, dk, p.scale, p.d, lane);
     if (p.dv.p) store_row<T, D>((T*)p.dv.p + b * p.dv.b + kh * p.dv.h + (long)j * p.dv.l, dv, 1.f, p.d, lane);
+  }
+}
+
+// dk, dv of the key tiles whose queries were split: the segments' sums in their order.  A block joins a quarter of a wave's part.
+template <typename T, int D> __global__ __launch_bounds__(256) void dkv_join_kernel(const Params p) {
+  constexpr int BM = BwdTile<T, D>::kRows, kPieces = D / 8;  // 16-byte pieces a lane: D / 32 blocks x 4, of dk and of dv
+  const int unit = blockIdx.x >> 2, w = blockIdx.x & 3, lane = threadIdx.x & 63;
+  const int tile = unit % p.k_tiles, bk = unit / p.k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
+  int t0, tiles;
+  query_tiles<BM>(p, tile, keys_of(p, b), start_of(p, b), &t0, &tiles);
+  const int all = tiles * p.G;
+  if (all <= p.seg_tiles) return;
+  const int segs = (all + p.seg_tiles - 1) / p.seg_tiles, j = tile * kRows + 32 * w + (lane & 31);
+  const float* part = p.part_o + ((long)unit * p.segs * 4 + w) * (2 * 32 * D) + lane * 4;
+  for (int n = threadIdx.x >> 6; n < 2 * kPieces; n += 4) {
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < segs; ++s) t += *reinterpret_cast<const f32x4*>(part + (long)s * 4 * (2 * 32 * D) + n * 256);
+    const bool value = n >= kPieces;
+    const View& o = value ? p.dv : p.dk;
+    const float f = value ? 1.f : p.scale;
+    const int e = value ? n - kPieces : n;
+    if (o.p && j < p.Lk) store4<T>((T*)o.p + b * o.b + kh * o.h + (long)j * o.l, e / 4 * 32 + 8 * (e & 3) + 4 * (lane >> 5), p.d, t[0] * f, t[1] * f, t[2] * f, t[3] * f);
   }
 }
 
@@ -345,16 +392,20 @@ template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p,
   OCEAN_TRY(set_lds(dq_kernel<T, D, BIAS, MASK>, lds));
   hipLaunchKernelGGL((dq_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
-  const int k_tiles = (p.Lk + kRows - 1) / kRows;
   if (p.dk.p || p.dv.p || p.dtable_part) {
     lds = 4 * BN * TL::kRowBytes + 4 * BN * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
     if (BIAS && p.dtable_part) lds += (4 * slots + 4 * 32 * 33) * sizeof(float);
     OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS, MASK>, lds));
-    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.Hk * k_tiles)), dim3(256), lds, s, p, k_tiles);
+    const long units = (long)p.B * p.Hk * p.k_tiles;
+    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)(units * p.segs)), dim3(256), lds, s, p);
     OCEAN_LAUNCH_CHECK();
+    if (p.segs > 1 && (p.dk.p || p.dv.p)) {
+      hipLaunchKernelGGL((dkv_join_kernel<T, D>), dim3((unsigned)(units * 4)), dim3(256), 0, s, p);
+      OCEAN_LAUNCH_CHECK();
+    }
   }
   if (BIAS && p.dtable_part) {
-    hipLaunchKernelGGL(dtable_kernel, dim3(p.H, p.buckets), dim3(256), 0, s, p.dtable_part, dtable, p.B * k_tiles, p.buckets, p.H);
+    hipLaunchKernelGGL(dtable_kernel, dim3(p.H, p.buckets), dim3(256), 0, s, p.dtable_part, dtable, p.B * p.k_tiles * p.segs, p.buckets, p.H);
     OCEAN_LAUNCH_CHECK();
   }
   return OCEAN_OK;

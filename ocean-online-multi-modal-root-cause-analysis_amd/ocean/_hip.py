@@ -196,12 +196,12 @@ def _declare_rest(lib) -> None:
     sig("ocean_gatconv_bwd_workspace", c_size_t, gp_)
     sig("ocean_gatconv_fwd", c_int, gp_, vp, tp, tp, vp, c_size_t, vp, vp)
     sig("ocean_gatconv_bwd", c_int, gp_, vp, tp, tp, vp, vp, vp, c_size_t, tp, vp, vp)
-    at_ = POINTER(AttentionShape)
+    at_ = c_void_p                       # an AttentionShape by reference, or its packed bytes
     sig("ocean_attention_fwd_workspace", c_size_t, at_)
     sig("ocean_attention_bwd_workspace", c_size_t, at_)
     sig("ocean_attention_fwd", c_int, at_, vp, vp, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp)
     sig("ocean_attention_bwd", c_int, at_, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp, vp, vp)
-    ln_ = POINTER(LayerNormShape)
+    ln_ = c_void_p                       # likewise
     sig("ocean_layer_norm_fwd", c_int, ln_, vp, vp, vp, vp, vp, vp, vp, vp)
     sig("ocean_layer_norm_bwd_workspace", c_size_t, ln_)
     sig("ocean_layer_norm_bwd", c_int, ln_, vp, vp, vp, vp, vp, vp, c_size_t, vp, vp, vp, vp)

@@ -6,14 +6,12 @@ stream.  None of them has a CPU path.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
-
-from torch.autograd.function import once_differentiable
 
 from . import _hip
 
@@ -380,19 +378,29 @@ def diversity_loss(x: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- sequences: attention without stored weights, layer norm
+# Small calls are bound by what the host does for them, so these two functions pack their shape structures in one step, ask
+# for the raw stream handle, and go around autograd where nothing needs a gradient.
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_pack_attention = struct.Struct("@9if4i28l").pack            # ocean_attention_shape
+_pack_norm = struct.Struct("@l2if4x4l").pack                 # ocean_layer_norm_shape
 
 
-def _on(device):
-    """The device guard of the sequence operators: their tensors may live on another GPU than the current one."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _stream_of(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _gpu(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
-    if not t.is_cuda:
+def _gpu(t: torch.Tensor, name: str, index: Optional[int] = None) -> int:
+    """The GPU `t` lives on, which must be number `index` if that is given."""
+    at = t.get_device()
+    if at < 0:
         raise _hip.OceanHipError(f"{name} must live on the GPU (got {t.device}); the HIP path has no CPU fallback")
-    if like is not None and t.device != like.device:
-        raise ValueError(f"{name} lives on {t.device}, the other inputs on {like.device}")
+    if index is not None and at != index:
+        raise ValueError(f"{name} lives on {t.device}, the other inputs on cuda:{index}")
+    return at
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _at(t: Optional[torch.Tensor]):
@@ -405,72 +413,82 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     return out if out.stride(-1) == 1 else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
-def _set_strides(field, t: torch.Tensor) -> None:
-    field[0], field[1], field[2] = t.stride(0), t.stride(1), t.stride(2)
+def _once() -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError("the backward pass of this operator cannot itself be differentiated (create_graph=True)")
+
+
+_NO_STRIDES = (0, 0, 0)
+
+
+def _attention_forward(q, k, v, mask, lengths, starts, table, cfg, want_lse):
+    """(out, lse or None, what the backward call packs again)"""
+    causal, start, scale, max_distance, both = cfg
+    out = _like(q)
+    if out.numel() == 0 or k.numel() == 0:
+        return out.zero_(), None, None
+    L = _hip.lib()
+    B, H, Lq, d = q.shape
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    head = (B, H, k.shape[1], Lq, k.shape[2], d, _DTYPES[q.dtype], causal, start, scale, 0 if table is None else table.shape[0], max_distance, both)
+    loose = (qp % 16 != 0) | (kp % 16 != 0) << 1 | (vp % 16 != 0) << 2
+    strides = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+    mask_strides = (0, 0, 0, 0) if mask is None else mask.stride()
+    sh = _pack_attention(*head, loose, *strides, *_NO_STRIDES, *_NO_STRIDES, *_NO_STRIDES, *_NO_STRIDES, *mask_strides)
+    dev = q.device
+    lse = torch.empty((B, H, Lq), device=dev, dtype=torch.float32) if want_lse else None
+    n = L.ocean_attention_fwd_workspace(sh)
+    ws = torch.empty(n, device=dev, dtype=torch.float32) if n else None
+    rc = L.ocean_attention_fwd(sh, qp, kp, vp, _at(mask), _at(lengths), _at(starts), _at(table), _at(ws), n, out.data_ptr(), _at(lse), _stream_of(dev))
+    if rc:
+        _hip.check(rc, "ocean_attention_fwd")
+    return out, lse, (head, loose, strides, mask_strides)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, lengths, starts, table, causal, start, scale, max_distance, both):
-        L = _hip.lib()
-        sh = _hip.AttentionShape()
-        sh.B, sh.H, sh.Lq, sh.d = q.shape
-        sh.Hk, sh.Lk = k.shape[1], k.shape[2]
-        sh.dtype, sh.causal, sh.query_start, sh.scale = _DTYPES[q.dtype], causal, start, scale
-        _set_strides(sh.q_strides, q)
-        _set_strides(sh.k_strides, k)
-        _set_strides(sh.v_strides, v)
-        if mask is not None:
-            for n, st in enumerate(mask.stride()):
-                sh.mask_strides[n] = st
-        if table is not None:
-            sh.num_buckets, sh.max_distance, sh.bidirectional = table.shape[0], max_distance, both
-        out = _like(q)
-        _set_strides(sh.o_strides, out)
-        sh.unaligned = (q.data_ptr() % 16 != 0) | (k.data_ptr() % 16 != 0) << 1 | (v.data_ptr() % 16 != 0) << 2
-        ctx.sh = sh
-        if q.numel() == 0 or k.numel() == 0:
-            ctx.save_for_backward(q, k, v, table)
-            return out.zero_()
-        train = any(ctx.needs_input_grad)
-        with _on(q.device):
-            lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32) if train else None
-            n = L.ocean_attention_fwd_workspace(ctypes.byref(sh))
-            ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-            _hip.check(L.ocean_attention_fwd(ctypes.byref(sh), _at(q), _at(k), _at(v), _at(mask), _at(lengths), _at(starts), _at(table),
-                                             _at(ws), n, _at(out), _at(lse), _hip.stream()), "ocean_attention_fwd")
-        if train:
-            ctx.save_for_backward(q, k, v, table, mask, lengths, starts, out, lse)
+    def forward(ctx, q, k, v, mask, lengths, starts, table, cfg):
+        out, lse, ctx.packed = _attention_forward(q, k, v, mask, lengths, starts, table, cfg, True)
+        ctx.save_for_backward(q, k, v, mask, lengths, starts, table, out, lse)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
+        _once()
+        q, k, v, mask, lengths, starts, table, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if lse is None:                                       # no query or no key: nothing depends on anything
+            dq, dk, dv, dt = (torch.zeros_like(t) if need[n] else None for n, t in ((0, q), (1, k), (2, v), (6, table)))
+            return dq, dk, dv, None, None, None, dt, None
         L = _hip.lib()
-        sh = ctx.sh
-        need = [ctx.needs_input_grad[n] for n in (0, 1, 2, 6)]
-        if len(ctx.saved_tensors) == 4:                       # no query or no key: nothing depends on anything
-            g = [torch.zeros_like(t) if n else None for n, t in zip(need, ctx.saved_tensors)]
-        else:
-            q, k, v, table, mask, lengths, starts, out, lse = ctx.saved_tensors
-            if d_out.stride(3) != 1:
-                d_out = d_out.contiguous()
-            g = [_like(t) if n else None for n, t in zip(need, (q, k, v, table))]
-            _set_strides(sh.go_strides, d_out)
-            sh.unaligned = sh.unaligned & 7 | (d_out.data_ptr() % 16 != 0) << 3
-            for field, t in zip((sh.dq_strides, sh.dk_strides, sh.dv_strides), g):
-                if t is not None:
-                    _set_strides(field, t)
-            with _on(q.device):
-                ws = torch.empty(L.ocean_attention_bwd_workspace(ctypes.byref(sh)), device=q.device, dtype=torch.float32)
-                _hip.check(L.ocean_attention_bwd(ctypes.byref(sh), _at(q), _at(k), _at(v), _at(mask), _at(lengths), _at(starts), _at(table),
-                                                 _at(out), _at(lse), _at(d_out), _at(ws), ws.numel(), _at(g[0]), _at(g[1]), _at(g[2]),
-                                                 _at(g[3]), _hip.stream()), "ocean_attention_bwd")
-        return g[0], g[1], g[2], None, None, None, g[3], None, None, None, None, None
+        dev = q.device
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                return _Attention.backward(ctx, d_out)
+        if d_out.stride(3) != 1:
+            d_out = d_out.contiguous()
+        dq, dk, dv, dt = (_like(t) if need[n] else None for n, t in ((0, q), (1, k), (2, v), (6, table)))
+        head, loose, strides, mask_strides = ctx.packed
+        gp = d_out.data_ptr()
+        st = lambda t: _NO_STRIDES if t is None else t.stride()[:3]
+        sh = _pack_attention(*head, loose | (gp % 16 != 0) << 3, *strides, *d_out.stride()[:3], *st(dq), *st(dk), *st(dv), *mask_strides)
+        n = L.ocean_attention_bwd_workspace(sh)
+        ws = lse.new_empty(n)
+        rc = L.ocean_attention_bwd(sh, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(mask), _at(lengths), _at(starts), _at(table), out.data_ptr(),
+                                   lse.data_ptr(), gp, ws.data_ptr(), n, _at(dq), _at(dk), _at(dv), _at(dt), _stream_of(dev))
+        if rc:
+            _hip.check(rc, "ocean_attention_bwd")
+        return dq, dk, dv, None, None, None, dt, None
 
 
-def _per_sample(t: torch.Tensor, name: str, B: int, like: torch.Tensor) -> torch.Tensor:
-    _gpu(t, name, like)
+def _attention(q, k, v, mask, lengths, starts, table, cfg):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+        return _Attention.apply(q, k, v, mask, lengths, starts, table, cfg)
+    return _attention_forward(q, k, v, mask, lengths, starts, table, cfg, False)[0]
+
+
+def _per_sample(t: torch.Tensor, name: str, B: int, index: int) -> torch.Tensor:
+    _gpu(t, name, index)
     if t.dtype != torch.int32 or t.shape != (B,):
         raise ValueError(f"{name} must be an int32 tensor of shape ({B},), got {t.dtype} {tuple(t.shape)}")
     return t.contiguous()
@@ -510,28 +528,28 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
         raise ValueError(f"attention takes fp32 or bf16 inputs of one type, got {query.dtype}, {key.dtype}, {value.dtype}")
     if not 1 <= d <= 128:
         raise ValueError(f"attention takes 1 to 128 features a head, got {d}")
-    _gpu(query, "query")
-    _gpu(key, "key", query)
-    _gpu(value, "value", query)
+    index = _gpu(query, "query")
+    _gpu(key, "key", index)
+    _gpu(value, "value", index)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not 0.0 < scale < 3.0e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if mask is not None:
-        _gpu(mask, "mask", query)
+        _gpu(mask, "mask", index)
         if mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"mask must be bool or uint8 (nonzero = allowed), got {mask.dtype}")
         mask = mask.view(torch.uint8).expand(B, H, Lq, Lk)
     if key_lengths is not None:
-        key_lengths = _per_sample(key_lengths, "key_lengths", B, query)
+        key_lengths = _per_sample(key_lengths, "key_lengths", B, index)
     starts, start = None, Lk - Lq
     if isinstance(query_start, torch.Tensor):
-        starts = _per_sample(query_start, "query_start", B, query)
+        starts = _per_sample(query_start, "query_start", B, index)
     elif query_start is not None:
         start = int(query_start)
     if not -(1 << 30) <= start <= (1 << 30):
         raise ValueError(f"query_start must be within 2^30, got {start}")
     if position_table is not None:
-        _gpu(position_table, "position_table", query)
+        _gpu(position_table, "position_table", index)
         if position_table.dim() != 2 or position_table.shape[1] != H or not position_table.is_floating_point():
             raise ValueError(f"position_table must be [buckets, {H}], got {tuple(position_table.shape)} {position_table.dtype}")
         nb = position_table.shape[0]
@@ -540,14 +558,19 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
             raise ValueError(f"2 to 128 buckets expected (an even number, 4 at least, when bidirectional), got {nb}")
         if not side // 2 < max_distance <= 2048:
             raise ValueError(f"max_distance must be above {side // 2} and at most 2048, got {max_distance}")
-        position_table = position_table.float().contiguous()
-    rows = lambda t: t if t.stride(3) == 1 else t.contiguous()
+        position_table = _fp32(position_table)
     least = 4 if query.dtype == torch.float32 else 8
     if d < least:                                             # the kernels read 16 bytes at a time
         pad = lambda t: torch.nn.functional.pad(t, (0, least - d))
         query, key, value = pad(query), pad(key), pad(value)
-    out = _Attention.apply(rows(query), rows(key), rows(value), mask, key_lengths, starts, position_table, int(bool(causal)), start, scale,
-                           int(max_distance), int(bool(bidirectional)))
+    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (query, key, value))
+    cfg = (int(bool(causal)), start, scale, int(max_distance), int(bool(bidirectional)))
+    args = (q, k, v, mask, key_lengths, starts, position_table, cfg)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            out = _attention(*args)
+    else:
+        out = _attention(*args)
     return out[..., :d] if d < least else out
 
 
@@ -562,100 +585,113 @@ def _row_stride(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t.contiguous(), W
 
 
+def _norm_forward(x, residual, weight, bias, eps, want_stats):
+    """(y, sum or None, the normalised rows, their stride, statistics or None)"""
+    W = x.shape[-1]
+    dev = x.device
+    y = x.new_empty(x.shape)
+    total = None if residual is None else x.new_empty(x.shape)
+    rows = x.numel() // W
+    if rows == 0:
+        return y, total, x, W, None
+    x, ldx = _row_stride(x)
+    residual, ldr = (None, 0) if residual is None else _row_stride(residual)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32) if want_stats else None
+    rc = _hip.lib().ocean_layer_norm_fwd(_pack_norm(rows, W, _DTYPES[y.dtype], eps, ldx, ldr, 0, 0), x.data_ptr(), _at(residual), _at(weight), _at(bias),
+                                         y.data_ptr(), _at(total), _at(stats), _stream_of(dev))
+    if rc:
+        _hip.check(rc, "ocean_layer_norm_fwd")
+    return (y, total, x, ldx, stats) if total is None else (y, total, total, W, stats)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps):
-        L = _hip.lib()
         ctx.set_materialize_grads(False)
-        sh = _hip.LayerNormShape()
-        W = x.shape[-1]
-        sh.rows, sh.width, sh.dtype, sh.eps = x.numel() // W, W, _DTYPES[x.dtype], eps
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        total = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        if x.numel() == 0:
-            ctx.save_for_backward(x if total is None else total, None, weight)
-        else:
-            train = any(ctx.needs_input_grad)
-            with _on(x.device):
-                xr, sh.x_stride = _row_stride(x)
-                rr = None
-                if residual is not None:
-                    rr, sh.residual_stride = _row_stride(residual)
-                stats = torch.empty(sh.rows, 2, device=x.device, dtype=torch.float32) if train else None
-                _hip.check(L.ocean_layer_norm_fwd(ctypes.byref(sh), _at(xr), _at(rr), _at(weight), _at(bias), _at(y), _at(total), _at(stats),
-                                                  _hip.stream()), "ocean_layer_norm_fwd")
-            if total is not None:
-                sh.x_stride = W
-            if train:
-                ctx.save_for_backward(xr if total is None else total, stats, weight)
-        ctx.sh, ctx.shape = sh, x.shape
+        y, total, rows, ctx.ldx, stats = _norm_forward(x, residual, weight, bias, eps, True)
+        ctx.save_for_backward(rows, stats, weight)
+        ctx.shape, ctx.eps = x.shape, eps
         return y if total is None else (y, total)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, d_sum=None):
+        _once()
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         if dy is None and d_sum is None:
             return None, None, None, None, None
-        L = _hip.lib()
-        sh = ctx.sh
         x, stats, weight = ctx.saved_tensors
-        if dy is None:                                        # only the sum was used
-            zeros = lambda n: torch.zeros(sh.width, device=x.device, dtype=torch.float32) if n else None
-            return d_sum if need_x else None, d_sum if need_r else None, zeros(need_w), zeros(need_b), None
-        dx = torch.empty(ctx.shape, device=x.device, dtype=x.dtype) if need_x or need_r else None
-        dw = torch.empty(sh.width, device=x.device, dtype=torch.float32) if need_w else None
-        db = torch.empty(sh.width, device=x.device, dtype=torch.float32) if need_b else None
-        if x.numel() == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        else:
-            with _on(x.device):
-                dyr, sh.dy_stride = _row_stride(dy)
-                dsr = None
-                if d_sum is not None:
-                    dsr, sh.dsum_stride = _row_stride(d_sum)
-                ws = torch.empty(L.ocean_layer_norm_bwd_workspace(ctypes.byref(sh)), device=x.device, dtype=torch.float32) \
-                    if need_w or need_b else None
-                _hip.check(L.ocean_layer_norm_bwd(ctypes.byref(sh), _at(x), _at(stats), _at(weight), _at(dyr), _at(dsr), _at(ws),
-                                                  0 if ws is None else ws.numel(), _at(dx), _at(dw), _at(db), _hip.stream()),
-                           "ocean_layer_norm_bwd")
+        W, dev = ctx.shape[-1], x.device
+        if dy is None or stats is None:                       # only the sum was used, or there are no rows
+            zeros = lambda n: torch.zeros(W, device=dev, dtype=torch.float32) if n else None
+            dx = d_sum if dy is None else torch.zeros(ctx.shape, device=dev, dtype=x.dtype)
+            return dx if need_x else None, dx if need_r else None, zeros(need_w), zeros(need_b), None
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                return _LayerNorm.backward(ctx, dy, d_sum)
+        L = _hip.lib()
+        dx = x.new_empty(ctx.shape) if need_x or need_r else None
+        dw = stats.new_empty(W) if need_w else None
+        db = stats.new_empty(W) if need_b else None
+        dy, ldy = _row_stride(dy)
+        d_sum, lds = (None, 0) if d_sum is None else _row_stride(d_sum)
+        sh = _pack_norm(x.numel() // W, W, _DTYPES[x.dtype], ctx.eps, ctx.ldx, 0, ldy, lds)
+        n = L.ocean_layer_norm_bwd_workspace(sh) if need_w or need_b else 0
+        ws = stats.new_empty(n) if n else None
+        rc = L.ocean_layer_norm_bwd(sh, x.data_ptr(), stats.data_ptr(), _at(weight), dy.data_ptr(), _at(d_sum), _at(ws), n, _at(dx), _at(dw), _at(db),
+                                    _stream_of(dev))
+        if rc:
+            _hip.check(rc, "ocean_layer_norm_bwd")
         return dx if need_x else None, dx if need_r else None, dw, db, None
 
 
-def _norm_args(x: torch.Tensor, residual, weight, bias, eps: float):
-    if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] > (1 << 24):
+def _norm_parameter(t: torch.Tensor, name: str, W: int, index: int) -> torch.Tensor:
+    _gpu(t, name, index)
+    if t.dim() != 1 or t.shape[0] != W or not t.is_floating_point():
+        raise ValueError(f"{name} must be [{W}], got {tuple(t.shape)} {t.dtype}")
+    return _fp32(t)
+
+
+def _norm(x, residual, weight, bias, eps):
+    W = x.shape[-1] if x.dim() else 0
+    if not 1 <= W <= 1 << 24:
         raise ValueError(f"layer_norm takes [..., width] with 1 to 2^24 columns, got {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
         raise ValueError(f"layer_norm takes fp32, bf16 or fp16 rows, got {x.dtype}")
-    _gpu(x, "x")
+    index = _gpu(x, "x")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
+    grad = x.requires_grad
     if residual is not None:
-        _gpu(residual, "residual", x)
+        _gpu(residual, "residual", index)
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"x and residual must agree in shape and type, got {tuple(x.shape)} {x.dtype}, {tuple(residual.shape)} {residual.dtype}")
-    out = []
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _gpu(t, name, x)
-            if t.shape != x.shape[-1:] or not t.is_floating_point():
-                raise ValueError(f"{name} must be [{x.shape[-1]}], got {tuple(t.shape)} {t.dtype}")
-            t = t.float().contiguous()
-        out.append(t)
-    return out
+        grad = grad or residual.requires_grad
+    if weight is not None:
+        weight = _norm_parameter(weight, "weight", W, index)
+        grad = grad or weight.requires_grad
+    if bias is not None:
+        bias = _norm_parameter(bias, "bias", W, index)
+        grad = grad or bias.requires_grad
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _norm_call(x, residual, weight, bias, float(eps), grad)
+    return _norm_call(x, residual, weight, bias, float(eps), grad)
+
+
+def _norm_call(x, residual, weight, bias, eps, grad):
+    if grad and torch.is_grad_enabled():
+        return _LayerNorm.apply(x, residual, weight, bias, eps)
+    y, total = _norm_forward(x, residual, weight, bias, eps, False)[:2]
+    return y if total is None else (y, total)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, any width, fp32, bf16 or fp16 (statistics and
     the weights' gradients in fp32, the latter summed in a fixed order); weight and bias [width] in any floating type, or None."""
-    weight, bias = _norm_args(x, None, weight, bias, eps)
-    return _LayerNorm.apply(x, None, weight, bias, float(eps))
+    return _norm(x, None, weight, bias, eps)
 
 
 def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                    eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
     """(layer_norm(s), s) with s = x + residual, rounded to their type, in one pass; the gradient of s joins the norm's."""
-    weight, bias = _norm_args(x, residual, weight, bias, eps)
-    return _LayerNorm.apply(x, residual, weight, bias, float(eps))
+    return _norm(x, residual, weight, bias, eps)
