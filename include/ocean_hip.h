@@ -587,7 +587,7 @@ typedef struct {
   int query_start;
   float scale;                     /* > 0 */
   int num_buckets;                 /* 0: no position bias; at most 128 */
-  int max_distance;                /* > E, at most 2048 */
+  int max_distance;                /* > E, at most 1024 */
   int bidirectional;
   int unaligned;                   /* bits 0..3: q, k, v, d_out do not begin on a 16-byte boundary (refused if they do not and the
                                       bit is missing); such inputs, and those of odd strides or d, are copied to the workspace */

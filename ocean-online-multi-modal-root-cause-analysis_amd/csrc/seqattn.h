@@ -24,7 +24,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kMaxDist = 2048;       // largest max_distance: 2 * 2048 + 1 biases of one head stay in LDS
+constexpr int kMaxDist = 1024;       // largest max_distance: a head's biases by distance, and four waves' sums of their gradients, stay in LDS
 constexpr int kMaxBuckets = 128;
 
 struct View { const void* p; long b, h, l; };            // element strides of batch, head, position; the feature's is 1
@@ -291,7 +291,8 @@ __device__ __forceinline__ int die_order(int id, int n) {
 }
 
 constexpr int kKeyTile = 128;        // keys of a block of the launch over keys
-constexpr int query_tile(bool bits16) { return bits16 ? 64 : 32; }       // and the queries it takes at a time
+constexpr int query_tile(int row_bytes) { return row_bytes <= 192 ? 64 : 32; }       // and the queries it takes at a time
+constexpr bool values_in_lds(int row_bytes) { return row_bytes >= 256 && row_bytes < 512; }
 
 int launch_forward(const Params& p, int type, hipStream_t s);
 int launch_backward(const Params& p, int type, float* dtable, hipStream_t s);

@@ -62,11 +62,11 @@ int pack(const ocean_attention_shape* s, View* v, const long* st, int bit, int h
 // and the partial sums were measured to take.
 void plan_segments(const ocean_attention_shape* s, int D, int* segs, int* seg_tiles) {
   const bool b16 = s->dtype != OCEAN_F32;
-  const int rows = seqattn::query_tile(b16);
+  const int rows = seqattn::query_tile(D * (b16 ? 2 : 4));
   const long units = (long)s->B * s->Hk * ((s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile);
   const long tiles = (long)(s->H / s->Hk) * ((s->Lq + rows - 1) / rows);
-  const double slots = D * (b16 ? 2 : 4) > 128 ? 256.0 : 512.0;
-  const double tile_us = (b16 ? 2.5 : 8.0) * D / 128.0 * (slots / 256.0);
+  const double slots = D * (b16 ? 2 : 4) > 256 ? 256.0 : 512.0;
+  const double tile_us = rows / 32 * (b16 ? 1.1 : 8.0) * D / 128.0 * (slots / 256.0);
   double best = 1e30;
   *segs = 1;
   for (int n = 1; n <= 16 && (n == 1 || n <= tiles / 2); ++n) {

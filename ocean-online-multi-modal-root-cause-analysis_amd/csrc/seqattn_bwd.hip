@@ -32,13 +32,17 @@ template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(co
   }
 }
 
-// Sums of a wave's 32x32 block of ds (rows: queries, own columns: keys) over its 63 diagonals, through LDS of the wave (pitch
-// 33: a diagonal is a fixed step), lane t taking distance d0 + t - 31; then into the wave's own sums by distance.  One lane owns one distance, and blocks follow
-// each other in order: the sums come out the same in every run.
+// Sums of a wave's 32x32 block of ds (rows: queries, own columns: keys) over its 63 diagonals.  Eight rows make a chain: shifted by
+// one lane before each row is added, so that lane l of the chain of rows 8c..8c+7 ends up with the diagonal key - query = l - 7 - 8c.
+// The chains' lanes are added to the wave's own sums by distance (LDS additions of one wave, which happen in the order of its
+// instructions, and in each of them one lane a distance): the sums come out the same in every run.  (Through an LDS image of the block, 48 LDS accesses a lane, the launch over keys took 111 us for 16 x 12 heads x 512 x 64,
+// this way 71.)
 struct DiagSums {
-  float* scratch;                    // [32][33]
   float* by_dist;                    // [2 max_dist + 1]
   float below, above;                // distances of -max_dist and less, max_dist and more
+  static __device__ __forceinline__ float next_lane(float x) {      // lane l gets lane l - 1's, lane 0 gets 0
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x138, 0xf, 0xf, true));
+  }
   __device__ __forceinline__ void add(const Params& p, const f32x16& ds, int d0, int lane) {
     if (d0 + 31 <= -p.max_dist || d0 - 31 >= p.max_dist) {
       float t = 0.f;
@@ -47,23 +51,30 @@ struct DiagSums {
       if (d0 < 0) below += t; else above += t;
       return;
     }
+    float chain[4];
+    float hi[4][4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * 33 + (lane & 31)] = ds[r];
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float t = 0.f;
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int j = i + lane - 31;
-      const float x = scratch[i * 33 + min(max(j, 0), 31)];
-      t += j >= 0 && j < 32 ? x : 0.f;
+      for (int c = 0; c < 4; ++c) {
+        // registers 4c + e: row 8c + e in the lower half, 8c + 4 + e in the upper one; both halves to lanes 0..31 over zeros
+        const float x = ds[4 * c + e];
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), 0u, false, false);
+        hi[c][e] = __builtin_bit_cast(float, (uint32_t)r[1]);
+        const float lo = __builtin_bit_cast(float, (uint32_t)r[0]);
+        chain[c] = e == 0 ? lo : next_lane(chain[c]) + lo;
+      }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) chain[c] = next_lane(chain[c]) + hi[c][e];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int dist = d0 + lane - 7 - 8 * c;              // lanes 39.. hold zeros
+      if (dist <= -p.max_dist) below += chain[c];
+      else if (dist >= p.max_dist) above += chain[c];
+      else if (lane < 39) __hip_atomic_fetch_add(by_dist + dist + p.max_dist, chain[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int dist = d0 + lane - 31;
-    if (dist <= -p.max_dist) below += t;
-    else if (dist >= p.max_dist) above += t;
-    else if (lane < 63) by_dist[dist + p.max_dist] += t;
   }
 };
 
@@ -94,11 +105,14 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
   __syncthreads();
 }
 
-template <typename T, int D> struct BwdTile { static constexpr int kRows = query_tile(sizeof(T) == 2); };
+template <typename T, int D> struct BwdTile {
+  static constexpr int kRows = query_tile(D * sizeof(T));   // queries at a time of the launch over keys
+  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;    // keys at a time of the launch over queries
+};
 
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
-  constexpr int BN = BwdTile<T, D>::kRows, NS = BN / 32;
+  constexpr int BN = BwdTile<T, D>::kKeys, NS = BN / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int kBuf = BN * TL::kRowBytes;                  // two buffers of keys, two of values
   char* const kt = smem;
@@ -210,22 +224,26 @@ template <int BM> __device__ __forceinline__ void query_tiles(const Params& p, i
   *tiles = first < p.Lq ? (p.Lq + BM - 1) / BM - *t0 : 0;
 }
 
-template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 128 ? 1 : 2) void dkv_kernel(const Params p) {
+// A wave keeps its 32 keys' dk and dv in registers, and the keys as right operand; the values too where that leaves room for two
+// waves on a SIMD, else they stay in LDS (VL): at 128 16-bit features the registers of both were 440, and half of the instructions
+// moved accumulators between the two register files.
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
+  constexpr bool VL = values_in_lds(D * sizeof(T));
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int kBuf = BM * TL::kRowBytes;                  // two buffers of queries, two of the outputs' gradients
   char* const qt = smem;
   char* const gt = smem + 2 * kBuf;
-  float* const rowv = reinterpret_cast<float*>(smem + 4 * BM * TL::kRowBytes);      // [2][lse, delta][BM]
+  char* const vt = smem + 4 * kBuf;                          // VL: the block's values
+  float* const rowv = reinterpret_cast<float*>(vt + (VL ? kRows * TL::kRowBytes : 0));      // [2][lse, delta][BM]
   float* const lut = rowv + 4 * BM;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h4 = 4 * (lane >> 5), slots = 2 * p.max_dist + 1;
   DiagSums diag;
-  float* const dist_sums = lut + slots;                     // [wave][slots], then the waves' scratch
+  float* const dist_sums = lut + slots;                     // [wave][slots]
   const bool sum_bias = BIAS && p.dtable_part != nullptr;
   if (BIAS) {
     diag.by_dist = dist_sums + w * slots;
-    diag.scratch = dist_sums + 4 * slots + w * 32 * 33;
     diag.below = diag.above = 0.f;
     if (sum_bias) for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
   }
@@ -238,7 +256,8 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   const bool live = j < keys;
   RowRegs<T, D> k, v;
   k.load(live ? (const T*)p.k.p + b * p.k.b + kh * p.k.h + (long)j * p.k.l : nullptr, p.d, lane);
-  v.load(live ? (const T*)p.v.p + b * p.v.b + kh * p.v.h + (long)j * p.v.l : nullptr, p.d, lane);
+  const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
+  if (!VL) v.load(live ? vb + (long)j * p.v.l : nullptr, p.d, lane);
   const float c = p.scale * kLog2e;
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
@@ -263,6 +282,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     Load::load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
   };
   if (u0 < u1) {
+    if (VL) Async<T, D, kRows, 256>::load(vt, vb, p.v.l, tile * kRows, keys, p.d, tid);
     load(u0, u0 & 1);
     if (BIAS) fill_bias(p, head0 + u0 / tiles, lut, tid, 256);
   }
@@ -282,7 +302,14 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         const int i0 = r0 + 32 * n;
         const float* lr = rowv + cur * 2 * BM + 32 * n + h4;
         f32x16 s = row_mma<T, D>(qt + cur * kBuf, 32 * n, lane, k, f32x16{});
-        const f32x16 dp = row_mma<T, D>(gt + cur * kBuf, 32 * n, lane, v, f32x16{});
+        f32x16 dp = f32x16{};
+        if (VL) {
+#pragma unroll
+          for (int st = 0; st < RowRegs<T, D>::kSteps; ++st)
+            dp = Mm<T>::mma(TL::row_frag(gt + cur * kBuf, 32 * n, st, lane), TL::row_frag(vt, 32 * w, st, lane), dp);
+        } else {
+          dp = row_mma<T, D>(gt + cur * kBuf, 32 * n, lane, v, dp);
+        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r >> 2) + (r & 3);
@@ -385,7 +412,7 @@ template <typename K> int set_lds(K kernel, size_t bytes) {
 
 template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p, float* dtable, hipStream_t s) {
   typedef Tile<T, D> TL;
-  constexpr int BN = BwdTile<T, D>::kRows;
+  constexpr int BN = BwdTile<T, D>::kKeys, BM = BwdTile<T, D>::kRows;
   const size_t slots = 2 * p.max_dist + 1;
   size_t lds = 4 * BN * TL::kRowBytes;
   if (BIAS) lds += slots * sizeof(float);
@@ -393,8 +420,8 @@ template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p,
   hipLaunchKernelGGL((dq_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
   if (p.dk.p || p.dv.p || p.dtable_part) {
-    lds = 4 * BN * TL::kRowBytes + 4 * BN * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
-    if (BIAS && p.dtable_part) lds += (4 * slots + 4 * 32 * 33) * sizeof(float);
+    lds = (4 * BM + (values_in_lds(D * sizeof(T)) ? kRows : 0)) * TL::kRowBytes + 4 * BM * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
+    if (BIAS && p.dtable_part) lds += 4 * slots * sizeof(float);
     OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS, MASK>, lds));
     const long units = (long)p.B * p.Hk * p.k_tiles;
     hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)(units * p.segs)), dim3(256), lds, s, p);

@@ -516,7 +516,7 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
     position_table [buckets, heads]: the learned bias of the distance key - query position, added to the scaled scores.
     bidirectional: half of the buckets for each sign; else keys after the query count as distance 0.  With E = half of one
     side's buckets, distances below E have a bucket each, the others share the rest in logarithmic steps up to max_distance
-    (at most 2048; 128 buckets at most)."""
+    (at most 1024; 128 buckets at most)."""
     if query.dim() != 4 or key.dim() != 4 or value.shape != key.shape:
         raise ValueError(f"query [batch, heads, queries, d] and key, value [batch, key heads, keys, d] expected, got {tuple(query.shape)}, "
                          f"{tuple(key.shape)}, {tuple(value.shape)}")
@@ -556,8 +556,8 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
         side = nb // 2 if bidirectional else nb
         if side < 2 or nb > 128 or (bidirectional and nb % 2):
             raise ValueError(f"2 to 128 buckets expected (an even number, 4 at least, when bidirectional), got {nb}")
-        if not side // 2 < max_distance <= 2048:
-            raise ValueError(f"max_distance must be above {side // 2} and at most 2048, got {max_distance}")
+        if not side // 2 < max_distance <= 1024:
+            raise ValueError(f"max_distance must be above {side // 2} and at most 1024, got {max_distance}")
         position_table = _fp32(position_table)
     least = 4 if query.dtype == torch.float32 else 8
     if d < least:                                             # the kernels read 16 bytes at a time

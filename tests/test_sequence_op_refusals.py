@@ -49,7 +49,7 @@ def test_arguments_with_the_tensors_on_the_gpu():
            dict(key_lengths=torch.tensor([1, 2], device="cuda")), dict(key_lengths=i32(1, 2, 3)), dict(query_start=i32(1)),
            dict(query_start=1 << 31), dict(position_table=table[:, :3]), dict(position_table=table[:31]), dict(position_table=table[:2]),
            dict(position_table=table[:1], bidirectional=False), dict(position_table=table, max_distance=8),
-           dict(position_table=table, max_distance=2049), dict(position_table=torch.zeros(130, 4, device="cuda"))]
+           dict(position_table=table, max_distance=1025), dict(position_table=torch.zeros(130, 4, device="cuda"))]
     for kw in bad:
         with pytest.raises(ValueError):
             ops.attention(q, k, v, **kw)
@@ -81,7 +81,7 @@ def attention_shape(**change):
 @pytest.mark.parametrize("change,status", [
     (dict(B=0), 1), (dict(H=3), 1), (dict(Lq=0), 1), (dict(Lk=-1), 1), (dict(dtype=2), 1), (dict(scale=0.0), 1), (dict(scale=float("nan")), 1),
     (dict(d=129), 2), (dict(d=3), 2), (dict(d=7, dtype=1), 2), (dict(query_start=(1 << 30) + 1), 2), (dict(num_buckets=7, bidirectional=1, max_distance=9), 1),
-    (dict(num_buckets=8, max_distance=4), 1), (dict(num_buckets=130, max_distance=200), 2), (dict(num_buckets=8, max_distance=2049), 2), (dict(), 4)])
+    (dict(num_buckets=8, max_distance=4), 1), (dict(num_buckets=130, max_distance=200), 2), (dict(num_buckets=8, max_distance=1025), 2), (dict(), 4)])
 def test_attention_status_codes(change, status):
     L, s = _hip.lib(), attention_shape(**change)
     none = [None] * 8
