@@ -87,8 +87,11 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
   if ((tid & 63) == 0) { diag.by_dist[0] += lo; diag.by_dist[slots - 1] += hi; }
   diag.below = diag.above = 0.f;
   __syncthreads();
-  for (int k = tid; k < p.buckets; k += 256) {
-    // bucket k holds the distances of n0..n1 steps to one side
+  for (int x = tid; x < slots; x += 256) dist_sums[x] = (dist_sums[x] + dist_sums[slots + x]) + (dist_sums[2 * slots + x] + dist_sums[3 * slots + x]);
+  __syncthreads();
+  // bucket k holds the distances of n0..n1 steps to one side: sixteen lanes add a bucket's
+  const int sub = tid & 15;
+  for (int k = tid >> 4; k < p.buckets; k += 16) {
     const int right = p.both && k >= p.side, f = right ? k - p.side : k;
     int n0 = f <= p.exact ? f : p.limits[f - p.exact - 1];
     const int n1 = f == p.side - 1 ? p.max_dist : f < p.exact ? f : p.limits[f - p.exact] - 1;
@@ -96,9 +99,10 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
     if (right) { n0 = max(n0, 1); x0 = p.max_dist + n0; x1 = p.max_dist + n1; }
     if (!p.both && f == 0) x1 = slots - 1;
     float t = 0.f;
-    for (int x = x0; x <= x1; ++x)
-      for (int v = 0; v < 4; ++v) t += dist_sums[v * slots + x];
-    part[k] = t;
+    for (int x = x0 + sub; x <= x1; x += 16) t += dist_sums[x];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    if (sub == 0) part[k] = t;
   }
   __syncthreads();
   for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
@@ -118,7 +122,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const kt = smem;
   char* const vt = smem + 2 * kBuf;
   float* const lut = reinterpret_cast<float*>(smem + 4 * BN * TL::kRowBytes);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int id = die_order(blockIdx.x, gridDim.x);
   const int tile = p.q_tiles - 1 - id % p.q_tiles, bh = id / p.q_tiles, b = bh / p.H, head = bh % p.H, kh = head / p.G;
   const int keys = keys_of(p, b), start = start_of(p, b);
@@ -216,6 +220,18 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   if (live && lane < 32) p.delta[((long)b * p.H + head) * p.Lq + i] = delta;
 }
 
+// a lane's sixteen rows' values from 32 consecutive ones (from its half's first on)
+__device__ __forceinline__ f32x16 row_values(const float* at) {
+  f32x16 x;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 q = *reinterpret_cast<const f32x4*>(at + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * g + e] = q[e];
+  }
+  return x;
+}
+
 // the tiles of BM queries that see some key of the tile: `tiles` from t0 on
 template <int BM> __device__ __forceinline__ void query_tiles(const Params& p, int tile, int keys, int start, int* t0, int* tiles) {
   int first = p.causal ? min(max(tile * kRows - start, 0), p.Lq) : 0;
@@ -238,7 +254,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const vt = smem + 4 * kBuf;                          // VL: the block's values
   float* const rowv = reinterpret_cast<float*>(vt + (VL ? kRows * TL::kRowBytes : 0));      // [2][lse, delta][BM]
   float* const lut = rowv + 4 * BM;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, h4 = 4 * (lane >> 5), slots = 2 * p.max_dist + 1;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), h4 = 4 * (lane >> 5), slots = 2 * p.max_dist + 1;
   DiagSums diag;
   float* const dist_sums = lut + slots;                     // [wave][slots]
   const bool sum_bias = BIAS && p.dtable_part != nullptr;
@@ -270,13 +286,15 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   const int all = tiles * p.G, u0 = min(seg * p.seg_tiles, all), u1 = min(u0 + p.seg_tiles, all);
   const int head0 = kh * p.G;
   typedef Async<T, D, BM, 256> Load;
-  float rv = 0.f;                                           // threads 0..BM-1: lse, BM..2BM-1: delta
+  float rv = 0.f;                                           // threads 0..BM-1: -lse, BM..2BM-1: -delta
+  const float row_unit = 1.f / c;
   const auto load = [&](int u, int buf) {
     const int head = head0 + u / tiles, r0 = (t0 + u % tiles) * BM;
     if (tid < 2 * BM) {
       const int i = r0 + tid % BM;
       const float* from = tid < BM ? p.lse : p.delta;
-      rv = i < p.Lq ? from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? INFINITY : 0.f;
+      rv = i < p.Lq ? -from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? -INFINITY : 0.f;
+      if (sizeof(T) == 2 && tid < BM) rv *= row_unit;
     }
     Load::load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
     Load::load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
@@ -301,20 +319,28 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       for (int n = 0; n < NS; ++n) {
         const int i0 = r0 + 32 * n;
         const float* lr = rowv + cur * 2 * BM + 32 * n + h4;
-        f32x16 s = row_mma<T, D>(qt + cur * kBuf, 32 * n, lane, k, f32x16{});
-        f32x16 dp = f32x16{};
-        if (VL) {
+        // the sums start at the row's -lse (in score units; 16 bits) and -delta, read from LDS where they are needed
+        f32x16 s = f32x16{};
+        if (sizeof(T) == 2) s = row_values(lr);
+        s = row_mma<T, D>(qt + cur * kBuf, 32 * n, lane, k, s);
+        f32x16 dp;
+        const auto form_dp = [&] {
+          dp = row_values(lr + BM);
+          if (VL) {
 #pragma unroll
-          for (int st = 0; st < RowRegs<T, D>::kSteps; ++st)
-            dp = Mm<T>::mma(TL::row_frag(gt + cur * kBuf, 32 * n, st, lane), TL::row_frag(vt, 32 * w, st, lane), dp);
-        } else {
-          dp = row_mma<T, D>(gt + cur * kBuf, 32 * n, lane, v, dp);
-        }
+            for (int st = 0; st < RowRegs<T, D>::kSteps; ++st)
+              dp = Mm<T>::mma(TL::row_frag(gt + cur * kBuf, 32 * n, st, lane), TL::row_frag(vt, 32 * w, st, lane), dp);
+          } else {
+            dp = row_mma<T, D>(gt + cur * kBuf, 32 * n, lane, v, dp);
+          }
+        };
+        if (!VL) form_dp();
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r >> 2) + (r & 3);
-          const float t = BIAS ? lut[dist_slot(p, j - (start + i0 + h4 + at))] - lr[at] : -lr[at];
-          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
+          float t = sizeof(T) == 2 ? 0.f : lr[at];
+          if (BIAS) t += lut[dist_slot(p, j - (start + i0 + h4 + at))];
+          s[r] = __builtin_amdgcn_exp2f(BIAS || sizeof(T) != 2 ? fmaf(s[r], c, t) : s[r] * c);
         }
         if (MASK || j0 + 32 > keys || (p.causal && i0 < wfull)) {
           const uint8_t* mcol = MASK ? p.mask + b * p.mb + head * p.mh + (long)j * p.mj + (long)(i0 + h4) * p.mi : nullptr;
@@ -329,10 +355,16 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         }
         PFrag<T> pf;
         pf.set(s);
+        if (VL) __builtin_amdgcn_sched_barrier(0);          // one product at a time: the registers hold no more than its operands
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) dv[db] = col_mma<D>(gt + cur * kBuf, 32 * n, db, lane, pf, dv[db]);
+        if (VL) {
+          __builtin_amdgcn_sched_barrier(0);
+          form_dp();
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= dp[r] - lr[BM + 8 * (r >> 2) + (r & 3)];
+        for (int r = 0; r < 16; ++r) s[r] *= dp[r];
         if (sum_bias) diag.add(p, s, j0 - (start + i0), lane);
         pf.set(s);
 #pragma unroll

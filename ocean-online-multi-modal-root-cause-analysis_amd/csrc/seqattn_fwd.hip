@@ -68,7 +68,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const kt = smem;
   char* const vt = smem + 2 * kBuf;
   float* const lut = reinterpret_cast<float*>(smem + 4 * BN * TL::kRowBytes);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int id = die_order(blockIdx.x, gridDim.x);
   const int tile = p.q_tiles - 1 - id % p.q_tiles, bh = id / p.q_tiles, b = bh / p.H, head = bh % p.H, kh = head / p.G;
   const int keys = keys_of(p, b), start = start_of(p, b);
@@ -141,7 +141,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256) void fwd_split_kernel(const Params p) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   char* const kt = smem + w * 2 * 32 * TL::kRowBytes;
   char* const vt = kt + 32 * TL::kRowBytes;
   uint8_t* const bmap = reinterpret_cast<uint8_t*>(smem + 8 * 32 * TL::kRowBytes);
