@@ -27,6 +27,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxDist = 1024;       // largest max_distance: a head's biases by distance, and four waves' sums of their gradients, stay in LDS
 constexpr int kMaxBuckets = 128;
 
+constexpr int kKeyTile = 128;        // keys of a block of the launch over keys
+constexpr int query_tile(int row_bytes) { return row_bytes <= 192 ? 64 : 32; }       // and the queries it takes at a time
+constexpr int key_tile(bool bits16) { return bits16 ? 64 : 32; }           // keys at a time of the launches over queries
+constexpr bool values_in_lds(int row_bytes) { return row_bytes >= 256 && row_bytes < 512; }
+
 struct View { const void* p; long b, h, l; };            // element strides of batch, head, position; the feature's is 1
 
 struct Params {
@@ -45,7 +50,8 @@ struct Params {
   float* dtable_part;                // [H][B][key tiles][segments][buckets]
   int k_tiles, segs, seg_tiles;      // launch over keys: tiles of 128 keys, segments of their queries, query tiles (of all heads) a segment
   int splits; float* part_o; float* part_ml;     // partial results of split sums
-  int q_tiles;
+  int q_tiles;                       // tiles of 128 queries (over split keys: chunks of 32 rows)
+  int parts, part_tiles;             // launches over queries: parts a query tile's keys are split into, key tiles a part
 };
 
 // ---------------------------------------------------------------- types
@@ -290,9 +296,54 @@ __device__ __forceinline__ int die_order(int id, int n) {
   return die * per + min(die, rem) + k;
 }
 
-constexpr int kKeyTile = 128;        // keys of a block of the launch over keys
-constexpr int query_tile(int row_bytes) { return row_bytes <= 192 ? 64 : 32; }       // and the queries it takes at a time
-constexpr bool values_in_lds(int row_bytes) { return row_bytes >= 256 && row_bytes < 512; }
+
+// Block number -> (key head of a sample, place in its list of `inner` blocks).  A die takes every eighth key head, so that the blocks
+// that share keys and values share an L2 and samples of unequal lengths spread over the dies.  With `causal` the lists go through place by place, over all key heads (of the die): they begin with the longest
+// loops, and the short ones fill the end (16 heads x 4096: 280 us key head by key head, 236 this way).
+__device__ __forceinline__ void work_of(const Params& p, int id, int blocks, int inner, int* bk, int* place) {
+  const int groups = p.B * p.Hk;
+  if (groups % 8 == 0) {
+    const int per = groups / 8, r = id >> 3;
+    *bk = (id & 7) + 8 * (p.causal ? r % per : r / inner);
+    *place = p.causal ? r / per : r % inner;
+  } else if (8 % groups == 0 && inner % (8 / groups) == 0) {
+    *bk = (id & 7) % groups;                               // one, two or four key heads: several dies share one's list
+    *place = (id >> 3) * (8 / groups) + (id & 7) / groups;
+  } else if (p.causal) {
+    *bk = id % groups;
+    *place = id / groups;
+  } else {
+    const int r = die_order(id, blocks);
+    *bk = r / inner;
+    *place = r % inner;
+  }
+}
+// launches over queries: the last query tiles have the most keys with `causal`
+__device__ __forceinline__ void rows_work(const Params& p, int id, int blocks, int* bh, int* tile, int* part) {
+  int bk, r;
+  work_of(p, id, blocks, p.G * p.q_tiles * p.parts, &bk, &r);
+  *tile = p.q_tiles - 1 - r / (p.G * p.parts);
+  r %= p.G * p.parts;
+  *bh = bk * p.G + r / p.parts;
+  *part = r % p.parts;
+}
+
+// tiles of BN keys that some query of a tile may see
+template <int BN> __device__ __forceinline__ int key_tiles(const Params& p, int tile, int keys, int start) {
+  const int end = p.causal ? min(keys, start + min((tile + 1) * kKeyTile, p.Lq)) : keys;
+  return end > 0 ? (end + BN - 1) / BN : 0;
+}
+
+// a wave's 32 rows of partial sums, in the matrix instructions' layout: 64 lanes x 16 bytes a piece, D / 8 pieces
+template <int D> __device__ __forceinline__ void store_part(float* part, const f32x16* acc, int lane) {
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(part + (db * 4 + g) * 256 + lane * 4) = f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+// and where piece n of lane's row goes: features part_feature(..).. + 3
+__device__ __forceinline__ int part_feature(int n, int lane) { return n / 4 * 32 + 8 * (n & 3) + 4 * (lane >> 5); }
 
 int launch_forward(const Params& p, int type, hipStream_t s);
 int launch_backward(const Params& p, int type, float* dtable, hipStream_t s);

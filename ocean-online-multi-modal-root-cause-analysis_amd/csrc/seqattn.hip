@@ -56,32 +56,27 @@ int pack(const ocean_attention_shape* s, View* v, const long* st, int bit, int h
   return OCEAN_OK;
 }
 
-// How many segments the queries of a key tile are split into.  One block holds a key tile's gradients in registers, so with few
-// key tiles, or with `causal` (where the first tile has all queries and the last ones next to none), the chip waits for the longest
-// block.  Segments cost a round trip of fp32 partial sums.  The estimate counts both, in microseconds, from what one query tile
-// and the partial sums were measured to take.
-void plan_segments(const ocean_attention_shape* s, int D, int* segs, int* seg_tiles) {
-  const bool b16 = s->dtype != OCEAN_F32;
-  const int rows = seqattn::query_tile(D * (b16 ? 2 : 4));
-  const long units = (long)s->B * s->Hk * ((s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile);
-  const long tiles = (long)(s->H / s->Hk) * ((s->Lq + rows - 1) / rows);
-  const double slots = D * (b16 ? 2 : 4) > 256 ? 256.0 : 512.0;
-  const double tile_us = rows / 32 * (b16 ? 1.1 : 8.0) * D / 128.0 * (slots / 256.0);
+// Into how many pieces the loop of every block is split.  A block holds its tile's result in registers, so with few tiles, or with
+// `causal` (where one tile's loop is long and another's next to nothing), the chip waits for the longest block.  Pieces cost a round
+// trip of fp32 partial sums and a launch that joins them.  The estimate counts both, in microseconds: `tile_us` for one step of the
+// loop with the chip full, 4 TB/s for the partial sums.
+void plan_pieces(long units, long steps, bool causal, double slots, double tile_us, double piece_bytes, int* pieces, int* per_piece) {
   double best = 1e30;
-  *segs = 1;
-  for (int n = 1; n <= 16 && (n == 1 || n <= tiles / 2); ++n) {
-    const long per = (tiles + n - 1) / n;
-    double load = s->causal ? 0.5 * units * tiles / slots : ceil(units * n / slots) * per;
-    if (s->causal) load = load + 0.25 * per > per ? load + 0.25 * per : per;
-    const double us = load * tile_us + (n > 1 ? 5.0 + (double)units * n * seqattn::kKeyTile * D * 16.0 / 4.0e6 : 0.0);
-    if (us < best) { best = us; *segs = n; }
+  *pieces = 1;
+  for (int n = 1; n <= 16 && (n == 1 || n <= steps / 2); ++n) {
+    const long per = (steps + n - 1) / n;
+    double load = causal ? 0.5 * units * steps / slots : ceil(units * n / slots) * per;
+    if (causal) load = load + 0.25 * per > per ? load + 0.25 * per : per;
+    const double us = load * tile_us + (n > 1 ? 5.0 + 2.0 * units * n * piece_bytes / 4.0e6 : 0.0);
+    if (us < best) { best = us; *pieces = n; }
   }
-  *seg_tiles = (int)((tiles + *segs - 1) / *segs);
+  *per_piece = (int)((steps + *pieces - 1) / *pieces);
 }
 
-struct Plan { int segs, seg_tiles; size_t part_at; int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
+struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
+  *pl = Plan{};
   if (!s) return OCEAN_ERR_NULL;
   if (s->B <= 0 || s->H <= 0 || s->Hk <= 0 || s->Lq <= 0 || s->Lk <= 0 || s->d <= 0 || s->H % s->Hk != 0) return OCEAN_ERR_BAD_SHAPE;
   if (s->dtype != OCEAN_F32 && s->dtype != OCEAN_BF16) return OCEAN_ERR_BAD_SHAPE;
@@ -97,7 +92,7 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   }
   pl->D = (s->d + 31) / 32 * 32;
   const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
-  if (blocks > 0x7fffffffL || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL / 16) return OCEAN_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffffL / 16 || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL / 16) return OCEAN_ERR_UNSUPPORTED;
   // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as rows.
   pl->split = (long)s->Lq * G <= 32;
   pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
@@ -120,10 +115,26 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const size_t rows = (size_t)s->B * s->H * s->Lq;
   pl->delta_at = at;
   pl->parts_at = at + ((rows + 3) & ~size_t(3));
-  plan_segments(s, pl->D, &pl->segs, &pl->seg_tiles);
+  // rates measured with the chip full: a step is 64 (32 in fp32) keys or queries of a tile of 128
+  const bool b16 = s->dtype != OCEAN_F32;
+  const int key_step = seqattn::key_tile(b16), row_bytes = pl->D * (b16 ? 2 : 4), query_step = seqattn::query_tile(row_bytes);
+  const double wide = pl->D / 128.0, slots = row_bytes > 256 ? 256.0 : 512.0;
+  const long key_steps = (s->Lk + key_step - 1) / key_step, query_steps = (long)G * ((s->Lq + query_step - 1) / query_step);
+  plan_pieces(blocks, key_steps, s->causal, 512.0, (b16 ? 2.7 : 9.0) * wide, 128.0 * pl->D * 4, &pl->parts, &pl->part_tiles);
+  plan_pieces(blocks, key_steps, s->causal, slots, (b16 ? 3.6 : 13.0 * slots / 512.0) * wide, 128.0 * pl->D * 4, &pl->dq_parts, &pl->dq_part_tiles);
+  plan_pieces((long)s->B * s->Hk * ((s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile), query_steps, s->causal, slots,
+              (b16 ? 2.9 * query_step / 32.0 : 17.0 * slots / 512.0) * wide, 128.0 * pl->D * 8, &pl->segs, &pl->seg_tiles);
+  if (!pl->split && pl->parts > 1) {
+    pl->ml_at = pl->fwd_floats + (size_t)blocks * pl->parts * 128 * pl->D;
+    pl->packed = pl->fwd_floats;
+    pl->fwd_floats = pl->ml_at + (size_t)blocks * pl->parts * 256;
+  }
   const size_t k_tiles = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;
   pl->part_at = pl->parts_at + (((size_t)s->B * s->H * k_tiles * pl->segs * (s->num_buckets > 0 ? s->num_buckets : 0) + 3) & ~size_t(3));
-  pl->bwd_floats = pl->part_at + (pl->segs > 1 ? (size_t)s->B * s->Hk * k_tiles * pl->segs * seqattn::kKeyTile * pl->D * 2 : 0);
+  // partial sums: the two launches use the same place one after the other
+  const size_t over_keys = pl->segs > 1 ? (size_t)s->B * s->Hk * k_tiles * pl->segs * seqattn::kKeyTile * pl->D * 2 : 0;
+  const size_t over_queries = pl->dq_parts > 1 ? (size_t)blocks * pl->dq_parts * (128 * pl->D + 256) : 0;
+  pl->bwd_floats = pl->part_at + (over_keys > over_queries ? over_keys : over_queries);
   return OCEAN_OK;
 }
 
@@ -172,6 +183,10 @@ int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const voi
     p.part_o = ws;
     p.part_ml = ws + rows * pl.D;
   } else {
+    p.parts = pl.parts;
+    p.part_tiles = pl.part_tiles;
+    p.part_o = ws + pl.packed;
+    p.part_ml = ws + pl.ml_at;
     OCEAN_TRY(pack(s, &p.k, s->k_strides, 1, s->Hk, s->Lk, &ws, (hipStream_t)stream));
     OCEAN_TRY(pack(s, &p.v, s->v_strides, 2, s->Hk, s->Lk, &ws, (hipStream_t)stream));
   }
@@ -192,6 +207,9 @@ int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const voi
   p.delta = ws + pl.delta_at;
   p.dtable_part = dtable ? ws + pl.parts_at : nullptr;
   p.part_o = ws + pl.part_at;
+  p.part_ml = ws + pl.part_at + (size_t)s->B * s->H * p.q_tiles * pl.dq_parts * 128 * pl.D;
+  p.parts = pl.dq_parts;
+  p.part_tiles = pl.dq_part_tiles;
   p.k_tiles = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;
   p.segs = pl.segs;
   p.seg_tiles = pl.seg_tiles;

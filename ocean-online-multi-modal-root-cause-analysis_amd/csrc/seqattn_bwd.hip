@@ -111,7 +111,7 @@ __device__ __forceinline__ void store_bias_sums(const Params& p, DiagSums& diag,
 
 template <typename T, int D> struct BwdTile {
   static constexpr int kRows = query_tile(D * sizeof(T));   // queries at a time of the launch over keys
-  static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;    // keys at a time of the launch over queries
+  static constexpr int kKeys = key_tile(sizeof(T) == 2);    // keys at a time of the launch over queries
 };
 
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
@@ -123,12 +123,15 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const vt = smem + 2 * kBuf;
   float* const lut = reinterpret_cast<float*>(smem + 4 * BN * TL::kRowBytes);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int id = die_order(blockIdx.x, gridDim.x);
-  const int tile = p.q_tiles - 1 - id % p.q_tiles, bh = id / p.q_tiles, b = bh / p.H, head = bh % p.H, kh = head / p.G;
+  int bh, tile, part;
+  rows_work(p, blockIdx.x, gridDim.x, &bh, &tile, &part);
+  const int b = bh / p.H, head = bh % p.H, kh = head / p.G;
   const int keys = keys_of(p, b), start = start_of(p, b);
   const int i0 = tile * kRows + 32 * w, i = i0 + (lane & 31), pos = start + i;
   const bool live = i < p.Lq;
   if (BIAS) fill_bias(p, head, lut, tid, 256);
+  const int tiles = key_tiles<BN>(p, tile, keys, start), u0 = part * p.part_tiles, u1 = min(u0 + p.part_tiles, tiles);
+  if (part > 0 && u0 >= u1) return;
   const T* kb = (const T*)p.k.p + b * p.k.b + kh * p.k.h;
   const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
   RowRegs<T, D> q, go;
@@ -147,24 +150,20 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   delta = other_half_sum(delta);
   float rest = 0.f;
   const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
-  int end = keys, wend = keys, wfull = keys;
-  if (p.causal) {
-    end = min(end, start + min(tile * kRows + kRows, p.Lq));
-    wend = min(wend, start + min(i0 + 32, p.Lq));
-    wfull = min(wfull, start + i0 + 1);
-  }
+  int wend = keys, wfull = keys;
+  if (p.causal) { wend = min(wend, start + min(i0 + 32, p.Lq)); wfull = min(wfull, start + i0 + 1); }
   const float c = p.scale * kLog2e;
   f32x16 acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
   typedef Async<T, D, BN, 256> Load;
-  const int tiles = end > 0 ? (end + BN - 1) / BN : 0;
-  if (tiles > 0) {
-    Load::load(kt, kb, p.k.l, 0, keys, p.d, tid);
-    Load::load(vt, vb, p.v.l, 0, keys, p.d, tid);
+  if (u0 < u1) {
+    Load::load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
+    Load::load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
   }
   // Up to two tiles of keys sit in the two buffers.  Rows of so few keys are where 16-bit rounding of `o` reaches dq through delta
-  // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first.
+  // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first
+  // (a part has two tiles at least, so they are never split).
   const bool few = sizeof(T) == 2 && tiles <= 2;
   if (few && tiles == 2) {
     Load::load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid);
@@ -184,12 +183,12 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     }
     delta = other_half_sum(sum);
   }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = u0; t < u1; ++t) {
     const int j0 = t * BN, cur = t & 1;
     if (!few) {
       wait_tiles();
       __syncthreads();
-      if (t + 1 < tiles) {
+      if (t + 1 < u1) {
         Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
         Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
       }
@@ -212,6 +211,16 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         for (int db = 0; db < D / 32; ++db) acc[db] = col_mma<D>(kt + cur * kBuf, 32 * n, db, lane, pf, acc[db]);
       }
     }
+  }
+  if (tiles > p.part_tiles) {
+    const long at = ((long)bh * p.q_tiles + tile) * p.parts + part;
+    store_part<D>(p.part_o + (at * 4 + w) * 32 * D, acc, lane);
+    if (sizeof(T) == 2) rest = other_half_sum(rest);
+    if (lane < 32) {
+      p.part_ml[at * 256 + 64 * w + lane] = delta;
+      p.part_ml[at * 256 + 64 * w + 32 + lane] = rest;
+    }
+    return;
   }
   if (live && p.dq.p) store_row<T, D>((T*)p.dq.p + b * p.dq.b + head * p.dq.h + (long)i * p.dq.l, acc, p.scale, p.d, lane);
   // In 16 bits `o` was rounded, and so were the weights that formed it: delta is a few 1e-3 of |do| |o| off.  The row's ds sum to
@@ -263,10 +272,11 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     diag.below = diag.above = 0.f;
     if (sum_bias) for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
   }
-  // Work list: key head by key head; for each, the first segment of every key tile, then the second, ..  With `causal` the first
-  // tiles have the most queries, so the large pieces start first and the small ones fill the gaps.
-  const int k_tiles = p.k_tiles, id = die_order(blockIdx.x, gridDim.x);
-  const int tile = id % k_tiles, seg = id / k_tiles % p.segs, bk = id / (k_tiles * p.segs), b = bk / p.Hk, kh = bk % p.Hk;
+  // a key head's list: the first segment of every key tile, then the second, ..; with `causal` the first tiles have the most queries
+  const int k_tiles = p.k_tiles;
+  int bk, place;
+  work_of(p, blockIdx.x, gridDim.x, k_tiles * p.segs, &bk, &place);
+  const int tile = place % k_tiles, seg = place / k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
   const int keys = keys_of(p, b), start = start_of(p, b);
   const int j0 = tile * kRows + 32 * w, j = j0 + (lane & 31);
   const bool live = j < keys;
@@ -383,19 +393,37 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   }
   if (seg > 0 && u0 >= u1) return;
   if (all > p.seg_tiles) {                                  // more than one segment: sums in the matrix instructions' layout
-    float* part = p.part_o + ((((long)bk * k_tiles + tile) * p.segs + seg) * 4 + w) * (2 * 32 * D) + lane * 4;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        *reinterpret_cast<f32x4*>(part + (db * 4 + g) * 256) = f32x4{dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]};
-        *reinterpret_cast<f32x4*>(part + 32 * D + (db * 4 + g) * 256) = f32x4{dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]};
-      }
+    float* part = p.part_o + ((((long)bk * k_tiles + tile) * p.segs + seg) * 4 + w) * (2 * 32 * D);
+    store_part<D>(part, dk, lane);
+    store_part<D>(part + 32 * D, dv, lane);
     return;
   }
   if (j < p.Lk) {                                           // keys past the sample's end get zeros
     if (p.dk.p) store_row<T, D>((T*)p.dk.p + b * p.dk.b + kh * p.dk.h + (long)j * p.dk.l, dk, p.scale, p.d, lane);
     if (p.dv.p) store_row<T, D>((T*)p.dv.p + b * p.dv.b + kh * p.dv.h + (long)j * p.dv.l, dv, 1.f, p.d, lane);
+  }
+}
+
+// dq and delta of the query tiles whose keys were split: the parts' sums in their order
+template <typename T, int D> __global__ __launch_bounds__(256) void dq_join_kernel(const Params p) {
+  const int unit = blockIdx.x >> 2, w = blockIdx.x & 3, lane = threadIdx.x & 63, r = lane & 31;
+  const int tile = unit % p.q_tiles, bh = unit / p.q_tiles, b = bh / p.H, head = bh % p.H, i = tile * kRows + 32 * w + r;
+  const int tiles = key_tiles<BwdTile<T, D>::kKeys>(p, tile, keys_of(p, b), start_of(p, b));
+  if (tiles <= p.part_tiles || i >= p.Lq) return;
+  const int parts = (tiles + p.part_tiles - 1) / p.part_tiles;
+  const float* from = p.part_o + ((long)unit * p.parts * 4 + w) * 32 * D + lane * 4;
+  T* out = (T*)p.dq.p + b * p.dq.b + head * p.dq.h + (long)i * p.dq.l;
+  if (p.dq.p)
+    for (int n = threadIdx.x >> 6; n < D / 8; n += 4) {
+      f32x4 t = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < parts; ++s) t += *reinterpret_cast<const f32x4*>(from + (long)s * 4 * 32 * D + n * 256);
+      store4<T>(out, part_feature(n, lane), p.d, t[0] * p.scale, t[1] * p.scale, t[2] * p.scale, t[3] * p.scale);
+    }
+  if (threadIdx.x < 32) {
+    const float* dr = p.part_ml + (long)unit * p.parts * 256 + 64 * w + r;
+    float delta = dr[0];
+    for (int s = 0; s < parts; ++s) delta += dr[s * 256 + 32];
+    p.delta[((long)b * p.H + head) * p.Lq + i] = delta;
   }
 }
 
@@ -417,7 +445,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void dkv_join_ker
     const View& o = value ? p.dv : p.dk;
     const float f = value ? 1.f : p.scale;
     const int e = value ? n - kPieces : n;
-    if (o.p && j < p.Lk) store4<T>((T*)o.p + b * o.b + kh * o.h + (long)j * o.l, e / 4 * 32 + 8 * (e & 3) + 4 * (lane >> 5), p.d, t[0] * f, t[1] * f, t[2] * f, t[3] * f);
+    if (o.p && j < p.Lk) store4<T>((T*)o.p + b * o.b + kh * o.h + (long)j * o.l, part_feature(e, lane), p.d, t[0] * f, t[1] * f, t[2] * f, t[3] * f);
   }
 }
 
@@ -449,8 +477,12 @@ template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p,
   size_t lds = 4 * BN * TL::kRowBytes;
   if (BIAS) lds += slots * sizeof(float);
   OCEAN_TRY(set_lds(dq_kernel<T, D, BIAS, MASK>, lds));
-  hipLaunchKernelGGL((dq_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
+  hipLaunchKernelGGL((dq_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles * p.parts)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
+  if (p.parts > 1) {
+    hipLaunchKernelGGL((dq_join_kernel<T, D>), dim3((unsigned)((long)p.B * p.H * p.q_tiles * 4)), dim3(256), 0, s, p);
+    OCEAN_LAUNCH_CHECK();
+  }
   if (p.dk.p || p.dv.p || p.dtable_part) {
     lds = (4 * BM + (values_in_lds(D * sizeof(T)) ? kRows : 0)) * TL::kRowBytes + 4 * BM * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
     if (BIAS && p.dtable_part) lds += 4 * slots * sizeof(float);

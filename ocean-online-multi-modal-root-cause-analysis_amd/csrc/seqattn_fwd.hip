@@ -58,7 +58,30 @@ template <bool BIAS, bool MASK> __device__ __forceinline__ void adjust(const Par
   }
 }
 
-template <typename T, int D> struct FwdTile { static constexpr int kKeys = sizeof(T) == 2 ? 64 : 32; };
+template <typename T, int D> struct FwdTile { static constexpr int kKeys = key_tile(sizeof(T) == 2); };
+
+// joins a query tile's parts: a block takes a wave's 32 rows, its four waves the pieces in turn
+template <typename T, int D> __global__ __launch_bounds__(256) void fwd_rows_join_kernel(const Params p) {
+  const int unit = blockIdx.x >> 2, w = blockIdx.x & 3, lane = threadIdx.x & 63, r = lane & 31;
+  const int tile = unit % p.q_tiles, bh = unit / p.q_tiles, b = bh / p.H, head = bh % p.H, i = tile * kRows + 32 * w + r;
+  const int tiles = key_tiles<FwdTile<T, D>::kKeys>(p, tile, keys_of(p, b), start_of(p, b));
+  if (tiles <= p.part_tiles || i >= p.Lq) return;
+  const int parts = (tiles + p.part_tiles - 1) / p.part_tiles;
+  const float* ml = p.part_ml + (long)unit * p.parts * 256 + 64 * w + r;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < parts; ++s) m = fmaxf(m, ml[s * 256]);
+  const float mref = m == -INFINITY ? 0.f : m;
+  for (int s = 0; s < parts; ++s) l += __builtin_amdgcn_exp2f(ml[s * 256] - mref) * ml[s * 256 + 32];
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const float* from = p.part_o + ((long)unit * p.parts * 4 + w) * 32 * D + lane * 4;
+  T* out = (T*)p.o.p + b * p.o.b + head * p.o.h + (long)i * p.o.l;
+  for (int n = threadIdx.x >> 6; n < D / 8; n += 4) {
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < parts; ++s) t += *reinterpret_cast<const f32x4*>(from + (long)s * 4 * 32 * D + n * 256) * __builtin_amdgcn_exp2f(ml[s * 256] - mref);
+    store4<T>(out, part_feature(n, lane), p.d, t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv);
+  }
+  if (p.lse && threadIdx.x < 32) p.lse[((long)b * p.H + head) * p.Lq + i] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
 
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void fwd_rows_kernel(const Params p) {
   typedef Tile<T, D> TL;
@@ -69,8 +92,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const vt = smem + 2 * kBuf;
   float* const lut = reinterpret_cast<float*>(smem + 4 * BN * TL::kRowBytes);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int id = die_order(blockIdx.x, gridDim.x);
-  const int tile = p.q_tiles - 1 - id % p.q_tiles, bh = id / p.q_tiles, b = bh / p.H, head = bh % p.H, kh = head / p.G;
+  int bh, tile, part;
+  rows_work(p, blockIdx.x, gridDim.x, &bh, &tile, &part);
+  const int b = bh / p.H, head = bh % p.H, kh = head / p.G;
   const int keys = keys_of(p, b), start = start_of(p, b);
   const int i0 = tile * kRows + 32 * w, i = i0 + (lane & 31), pos = start + i;
   if (BIAS) fill_bias(p, head, lut, tid, 256);
@@ -80,10 +104,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   RowRegs<T, D> q;
   q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
   const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
-  int end = keys;                                           // keys that some query of the block may see
-  if (p.causal) end = min(end, start + min(tile * kRows + kRows, p.Lq));
-  int wend = keys;                                          // .. of this wave; below wfull no place of the wave is behind the diagonal
-  int wfull = keys;
+  const int tiles = key_tiles<BN>(p, tile, keys, start), u0 = part * p.part_tiles, u1 = min(u0 + p.part_tiles, tiles);
+  if (part > 0 && u0 >= u1) return;
+  int wend = keys, wfull = keys;                            // keys that some query of the wave sees; that every one does
   if (p.causal) { wend = min(wend, start + min(i0 + 32, p.Lq)); wfull = min(wfull, start + i0 + 1); }
   const float c = p.scale * kLog2e;
   const float mult = BIAS ? 1.f : c;
@@ -92,16 +115,15 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
   typedef Async<T, D, BN, 256> Load;
-  const int tiles = end > 0 ? (end + BN - 1) / BN : 0;
-  if (tiles > 0) {
-    Load::load(kt, kb, p.k.l, 0, keys, p.d, tid);
-    Load::load(vt, vb, p.v.l, 0, keys, p.d, tid);
+  if (u0 < u1) {
+    Load::load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
+    Load::load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
   }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = u0; t < u1; ++t) {
     const int j0 = t * BN, cur = t & 1;
     wait_tiles();
     __syncthreads();
-    if (t + 1 < tiles) {
+    if (t + 1 < u1) {
       Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
       Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
     }
@@ -127,8 +149,18 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       }
     }
   }
+  const float lsum = other_half_sum(st.l);
+  if (tiles > p.part_tiles) {
+    const long at = ((long)bh * p.q_tiles + tile) * p.parts + part;
+    store_part<D>(p.part_o + (at * 4 + w) * 32 * D, acc, lane);
+    if (lane < 32) {
+      p.part_ml[at * 256 + 64 * w + lane] = st.m;
+      p.part_ml[at * 256 + 64 * w + 32 + lane] = lsum;
+    }
+    return;
+  }
   if (live) {
-    const float l = other_half_sum(st.l);
+    const float l = lsum;
     store_row<T, D>((T*)p.o.p + b * p.o.b + head * p.o.h + (long)i * p.o.l, acc, l > 0.f || l != l ? 1.f / l : 0.f, p.d, lane);
     if (p.lse && lane < 32) p.lse[((long)b * p.H + head) * p.Lq + i] = l == 0.f ? INFINITY : st.m + __builtin_amdgcn_logf(l);
   }
@@ -292,8 +324,12 @@ template <typename T, int D, bool BIAS, bool MASK> int forward(const Params& p, 
   if (p.splits == 0) {
     const size_t lds = 4 * FwdTile<T, D>::kKeys * TL::kRowBytes + (BIAS ? (2 * p.max_dist + 1) * sizeof(float) : 0);
     OCEAN_TRY(set_lds(fwd_rows_kernel<T, D, BIAS, MASK>, lds));
-    hipLaunchKernelGGL((fwd_rows_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles)), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((fwd_rows_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.H * p.q_tiles * p.parts)), dim3(256), lds, s, p);
     OCEAN_LAUNCH_CHECK();
+    if (p.parts > 1) {
+      hipLaunchKernelGGL((fwd_rows_join_kernel<T, D>), dim3((unsigned)((long)p.B * p.H * p.q_tiles * 4)), dim3(256), 0, s, p);
+      OCEAN_LAUNCH_CHECK();
+    }
     return OCEAN_OK;
   }
   size_t lds = 8 * 32 * TL::kRowBytes + (BIAS ? 2 * p.max_dist + 1 : 0);
