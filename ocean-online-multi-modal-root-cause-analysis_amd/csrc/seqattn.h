@@ -183,18 +183,36 @@ template <typename T, int D, int ROWS, int THREADS> struct Stage {
 static __device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
 template <typename T, int D, int ROWS, int THREADS> struct Async {
   typedef Tile<T, D> TL;
-  static constexpr int kN = ROWS * TL::kCh / THREADS, E = Mm<T>::kEpc;
+  static constexpr int kN = ROWS * TL::kCh / THREADS, E = Mm<T>::kEpc, kStep = THREADS / TL::kCh;
   static_assert(ROWS * TL::kCh % THREADS == 0, "a tile is whole rounds of the block");
-  static __device__ __forceinline__ void load(char* t, const T* base, long stride, int row0, int rows, int d, int tid) {
-    char* const to = t + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
-    const bool inside = row0 + ROWS <= rows;
+  // every round kStep rows further at the same chunk, so that a lane has one offset and the rounds differ by a scalar
+  static constexpr bool kEven = THREADS % TL::kCh == 0 && kStep % 8 == 0;
+  long off[kEven ? 1 : kN];
+  __device__ __forceinline__ Async(long stride, int tid) {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const int id = tid + n * THREADS, row = id / TL::kCh, c = (id % TL::kCh) ^ TL::swz(row);
-      const T* from = base + (long)(row0 + row) * stride + c * E;
-      if (!(inside || row0 + row < rows) || c * E >= d) from = reinterpret_cast<const T*>(kZeros);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)(to + n * THREADS * 16), 16, 0, 0);
+    for (int n = 0; n < (kEven ? 1 : kN); ++n) {
+      const int id = tid + n * THREADS, row = id / TL::kCh;
+      off[n] = (long)row * stride + ((id % TL::kCh) ^ TL::swz(row)) * E;
     }
+  }
+  __device__ __forceinline__ void load(char* t, const T* base, long stride, int row0, int rows, int d, int tid) const {
+    char* const to = t + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+    const T* const first = base + (long)row0 * stride;
+    if (row0 + ROWS <= rows && d == D) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) issue(kEven ? first + (long)n * kStep * stride + off[0] : first + off[kEven ? 0 : n], to + n * THREADS * 16);
+    } else {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const int id = tid + n * THREADS, row = id / TL::kCh, c = (id % TL::kCh) ^ TL::swz(row);
+        const T* from = kEven ? first + (long)n * kStep * stride + off[0] : first + off[kEven ? 0 : n];
+        if (row0 + row >= rows || c * E >= d) from = reinterpret_cast<const T*>(kZeros);
+        issue(from, to + n * THREADS * 16);
+      }
+    }
+  }
+  static __device__ __forceinline__ void issue(const T* from, char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   }
 };
 // every load into LDS of this wave has arrived (vmcnt 0; the other counters are left alone)

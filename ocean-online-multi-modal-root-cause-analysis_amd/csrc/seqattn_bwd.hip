@@ -156,18 +156,18 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   f32x16 acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
-  typedef Async<T, D, BN, 256> Load;
+  const Async<T, D, BN, 256> kload(p.k.l, tid), vload(p.v.l, tid);
   if (u0 < u1) {
-    Load::load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
-    Load::load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
+    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
+    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
   }
   // Up to two tiles of keys sit in the two buffers.  Rows of so few keys are where 16-bit rounding of `o` reaches dq through delta
   // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first
   // (a part has two tiles at least, so they are never split).
   const bool few = sizeof(T) == 2 && tiles <= 2;
   if (few && tiles == 2) {
-    Load::load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid);
-    Load::load(vt + kBuf, vb, p.v.l, BN, keys, p.d, tid);
+    kload.load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid);
+    vload.load(vt + kBuf, vb, p.v.l, BN, keys, p.d, tid);
   }
   if (few) {
     wait_tiles();
@@ -189,8 +189,8 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       wait_tiles();
       __syncthreads();
       if (t + 1 < u1) {
-        Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
-        Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
+        kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
+        vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
       }
     }
     if (j0 < wend) {
@@ -295,7 +295,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   query_tiles<BM>(p, tile, keys, start, &t0, &tiles);
   const int all = tiles * p.G, u0 = min(seg * p.seg_tiles, all), u1 = min(u0 + p.seg_tiles, all);
   const int head0 = kh * p.G;
-  typedef Async<T, D, BM, 256> Load;
+  const Async<T, D, BM, 256> qload(p.q.l, tid), gload(p.go.l, tid);
   float rv = 0.f;                                           // threads 0..BM-1: -lse, BM..2BM-1: -delta
   const float row_unit = 1.f / c;
   const auto load = [&](int u, int buf) {
@@ -306,11 +306,11 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       rv = i < p.Lq ? -from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? -INFINITY : 0.f;
       if (sizeof(T) == 2 && tid < BM) rv *= row_unit;
     }
-    Load::load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
-    Load::load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
+    qload.load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
+    gload.load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
   };
   if (u0 < u1) {
-    if (VL) Async<T, D, kRows, 256>::load(vt, vb, p.v.l, tile * kRows, keys, p.d, tid);
+    if (VL) Async<T, D, kRows, 256>(p.v.l, tid).load(vt, vb, p.v.l, tile * kRows, keys, p.d, tid);
     load(u0, u0 & 1);
     if (BIAS) fill_bias(p, head0 + u0 / tiles, lut, tid, 256);
   }

@@ -114,18 +114,18 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   f32x16 acc[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
-  typedef Async<T, D, BN, 256> Load;
+  const Async<T, D, BN, 256> kload(p.k.l, tid), vload(p.v.l, tid);
   if (u0 < u1) {
-    Load::load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
-    Load::load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
+    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
+    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
   }
   for (int t = u0; t < u1; ++t) {
     const int j0 = t * BN, cur = t & 1;
     wait_tiles();
     __syncthreads();
     if (t + 1 < u1) {
-      Load::load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
-      Load::load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
+      kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
+      vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
     }
     if (j0 < wend) {
       f32x16 s[NS];
