@@ -315,6 +315,26 @@ __device__ __forceinline__ int die_order(int id, int n) {
 }
 
 
+// The biases of a lane's sixteen places of a 32x32 block, place r at distance first + step * (8 (r >> 2) + (r & 3)), where d0 is
+// the distance at the block's corner (d0 - 31 .. d0 + 31 occur): beyond max_dist there is one bias for all, and a block inside needs no
+// clamping, so its reads differ by constants.
+template <int STEP> __device__ __forceinline__ f32x16 block_bias(const Params& p, const float* lut, int first, int d0) {
+  f32x16 x;
+  if (d0 + 31 <= -p.max_dist || d0 - 31 >= p.max_dist) {
+    const float far = lut[d0 < 0 ? 0 : 2 * p.max_dist];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = far;
+  } else if (d0 - 31 >= -p.max_dist && d0 + 31 <= p.max_dist) {
+    const float* at = lut + p.max_dist + first + (STEP < 0 ? 27 * STEP : 0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = at[(STEP < 0 ? -27 * STEP : 0) + STEP * (8 * (r >> 2) + (r & 3))];
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = lut[dist_slot(p, first + STEP * (8 * (r >> 2) + (r & 3)))];
+  }
+  return x;
+}
+
 // Block number -> (key head of a sample, place in its list of `inner` blocks).  A die takes every eighth key head, so that the blocks
 // that share keys and values share an L2 and samples of unequal lengths spread over the dies.  With `causal` the lists go through place by place, over all key heads (of the die): they begin with the longest
 // loops, and the short ones fill the end (16 heads x 4096: 280 us key head by key head, 236 this way).

@@ -11,15 +11,18 @@ namespace {
 
 constexpr int kRows = kKeyTile;      // queries (keys) of a block: four waves, 32 each
 
-// p_ij for keys j0.. of this lane's query, from scores
-template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int keys,
-                                                                   const uint8_t* mrow, const float* lut, bool edge, int lane) {
+// p_ij for keys j0.. of this lane's query (at pos; the wave's first at pos0), from scores
+template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(const Params& p, f32x16& s, float c, float lse, int j0, int pos, int pos0, int keys,
+                                                                              const uint8_t* mrow, const float* lut, bool edge, int lane) {
   const int h4 = 4 * (lane >> 5);
+  f32x16 t;
+  if (BIAS) {
+    t = block_bias<1>(p, lut, j0 + h4 - pos, j0 - pos0);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const float t = BIAS ? lut[dist_slot(p, j0 + 8 * (r >> 2) + h4 + (r & 3) - pos)] - lse : -lse;
-    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, t));
+    for (int r = 0; r < 16; ++r) t[r] -= lse;
   }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, BIAS ? t[r] : -lse));
   if (MASK || edge) {
     const int end = (p.causal ? min(keys, pos + 1) : keys) - j0 - h4;
 #pragma unroll
@@ -177,7 +180,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       const int at = j / BN * kBuf, row = j % BN;
       f32x16 s = row_mma<T, D>(kt + at, row, lane, q, f32x16{});
       const f32x16 dp = row_mma<T, D>(vt + at, row, lane, go, f32x16{});
-      probabilities<BIAS, MASK>(p, s, c, lse, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
+      probabilities<BIAS, MASK>(p, s, c, lse, j, pos, start + i0, keys, mrow, lut, j + 32 > wfull, lane);
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum = fmaf(s[r], dp[r], sum);
     }
@@ -199,7 +202,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         const int j = j0 + 32 * n;
         f32x16 s = row_mma<T, D>(kt + cur * kBuf, 32 * n, lane, q, f32x16{});
         const f32x16 dp = row_mma<T, D>(vt + cur * kBuf, 32 * n, lane, go, f32x16{});
-        probabilities<BIAS, MASK>(p, s, c, lse, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
+        probabilities<BIAS, MASK>(p, s, c, lse, j, pos, start + i0, keys, mrow, lut, j + 32 > wfull, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] *= dp[r] - delta;
@@ -345,11 +348,13 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
           }
         };
         if (!VL) form_dp();
+        f32x16 bias;
+        if (BIAS) bias = block_bias<-1>(p, lut, j - (start + i0 + h4), j0 - (start + i0));
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r >> 2) + (r & 3);
           float t = sizeof(T) == 2 ? 0.f : lr[at];
-          if (BIAS) t += lut[dist_slot(p, j - (start + i0 + h4 + at))];
+          if (BIAS) t += bias[r];
           s[r] = __builtin_amdgcn_exp2f(BIAS || sizeof(T) != 2 ? fmaf(s[r], c, t) : s[r] * c);
         }
         if (MASK || j0 + 32 > keys || (p.causal && i0 < wfull)) {

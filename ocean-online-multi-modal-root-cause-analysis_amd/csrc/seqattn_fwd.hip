@@ -39,12 +39,13 @@ template <int N> __device__ __forceinline__ float softmax_step(f32x16 (&s)[N], f
 }
 
 // adds the bias and takes out the places that are not allowed, for keys j0..j0+31 and this lane's query
-template <bool BIAS, bool MASK> __device__ __forceinline__ void adjust(const Params& p, f32x16& s, float mult, int j0, int pos, int keys, const uint8_t* mrow,
-                                                             const float* lut, bool edge, int lane) {
+template <bool BIAS, bool MASK> __device__ __forceinline__ void adjust(const Params& p, f32x16& s, float mult, int j0, int pos, int pos0, int keys,
+                                                                        const uint8_t* mrow, const float* lut, bool edge, int lane) {
   const int h4 = 4 * (lane >> 5);
   if (BIAS) {
+    const f32x16 bias = block_bias<1>(p, lut, j0 + h4 - pos, j0 - pos0);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mult, lut[dist_slot(p, j0 + 8 * (r >> 2) + h4 + (r & 3) - pos)]);
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mult, bias[r]);
   }
   if (MASK || edge) {
     const int end = (p.causal ? min(keys, pos + 1) : keys) - j0 - h4;
@@ -133,7 +134,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       for (int n = 0; n < NS; ++n) {
         s[n] = row_mma<T, D>(kt + cur * kBuf, 32 * n, lane, q, f32x16{});
         const int j = j0 + 32 * n;
-        adjust<BIAS, MASK>(p, s[n], c, j, pos, keys, mrow, lut, j + 32 > wfull, lane);
+        adjust<BIAS, MASK>(p, s[n], c, j, pos, start + i0, keys, mrow, lut, j + 32 > wfull, lane);
       }
       const float f = softmax_step<NS>(s, mult, st);
       if (__any(f != 1.f)) {
@@ -226,7 +227,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
         s[0][r] = fmaf(s[0][r], c, p.table[(long)bmap[dist_slot(p, dist)] * p.H + min(head, p.H - 1)] * kLog2e);
       }
     }
-    adjust<false, MASK>(p, s[0], c, j0, pos, keys, mrow, nullptr, j0 + 32 > full, lane);
+    adjust<false, MASK>(p, s[0], c, j0, pos, 0, keys, mrow, nullptr, j0 + 32 > full, lane);
     const float f = softmax_step<1>(s, mult, st);
     if (__any(f != 1.f)) {
 #pragma unroll
