@@ -37,9 +37,10 @@ template <bool BIAS, bool MASK> __device__ __forceinline__ void probabilities(co
 
 // Sums of a wave's 32x32 block of ds (rows: queries, own columns: keys) over its 63 diagonals.  Eight rows make a chain: shifted by
 // one lane before each row is added, so that lane l of the chain of rows 8c..8c+7 ends up with the diagonal key - query = l - 7 - 8c.
-// The chains' lanes are added to the wave's own sums by distance (LDS additions of one wave, which happen in the order of its
-// instructions, and in each of them one lane a distance): the sums come out the same in every run.  (Through an LDS image of the block, 48 LDS accesses a lane, the launch over keys took 111 us for 16 x 12 heads x 512 x 64,
-// this way 71.)
+// The four chains are moved onto each other, lane l holding the diagonal l - 31, and added to the wave's own sums by distance: one
+// lane owns one distance and blocks follow each other in order, so the sums come out the same in every run.  (16 x 12 heads x
+// 512 x 64, launch over keys: 107 us through an LDS image of the block, 92 with LDS additions of the four chains, 71 this way; 57 is
+// the launch without the sums.)
 struct DiagSums {
   float* by_dist;                    // [2 max_dist + 1]
   float below, above;                // distances of -max_dist and less, max_dist and more
@@ -71,13 +72,15 @@ struct DiagSums {
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int c = 0; c < 4; ++c) chain[c] = next_lane(chain[c]) + hi[c][e];
+    float t = chain[3];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int dist = d0 + lane - 7 - 8 * c;              // lanes 39.. hold zeros
-      if (dist <= -p.max_dist) below += chain[c];
-      else if (dist >= p.max_dist) above += chain[c];
-      else if (lane < 39) __hip_atomic_fetch_add(by_dist + dist + p.max_dist, chain[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    }
+    for (int c = 0; c < 3; ++c)                             // chains are zero from lane 39 on, where the moves wrap to
+      t += __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * (lane - 8 * (3 - c)), __builtin_bit_cast(int, chain[c])));
+    const int dist = d0 + lane - 31;
+    if (dist <= -p.max_dist) below += t;
+    else if (dist >= p.max_dist) above += t;
+    else if (lane < 63) by_dist[dist + p.max_dist] += t;
+    asm volatile("" ::: "memory");                          // the next block's lanes own other distances: its reads stay behind these writes
   }
 };
 
