@@ -262,6 +262,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
   constexpr bool VL = values_in_lds(D * sizeof(T));
+  // 16 bits: the products start at -lse in score units (4e-6 of a probability, far below its rounding); the bias, whose gradient is
+  // summed in fp32, takes lse as it is
+  constexpr bool FROM_LSE = sizeof(T) == 2 && !BIAS;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int kBuf = BM * TL::kRowBytes;                  // two buffers of queries, two of the outputs' gradients
   char* const qt = smem;
@@ -310,7 +313,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       const int i = r0 + tid % BM;
       const float* from = tid < BM ? p.lse : p.delta;
       rv = i < p.Lq ? -from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? -INFINITY : 0.f;
-      if (sizeof(T) == 2 && tid < BM) rv *= row_unit;
+      if (FROM_LSE && tid < BM) rv *= row_unit;
     }
     qload.load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
     gload.load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
@@ -335,9 +338,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       for (int n = 0; n < NS; ++n) {
         const int i0 = r0 + 32 * n;
         const float* lr = rowv + cur * 2 * BM + 32 * n + h4;
-        // the sums start at the row's -lse (in score units; 16 bits) and -delta, read from LDS where they are needed
+        // the sums start at the row's -lse and -delta, read from LDS where they are needed
         f32x16 s = f32x16{};
-        if (sizeof(T) == 2) s = row_values(lr);
+        if (FROM_LSE) s = row_values(lr);
         s = row_mma<T, D>(qt + cur * kBuf, 32 * n, lane, k, s);
         f32x16 dp;
         const auto form_dp = [&] {
@@ -356,9 +359,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int at = 8 * (r >> 2) + (r & 3);
-          float t = sizeof(T) == 2 ? 0.f : lr[at];
+          float t = FROM_LSE ? 0.f : lr[at];
           if (BIAS) t += bias[r];
-          s[r] = __builtin_amdgcn_exp2f(BIAS || sizeof(T) != 2 ? fmaf(s[r], c, t) : s[r] * c);
+          s[r] = __builtin_amdgcn_exp2f(FROM_LSE ? s[r] * c : fmaf(s[r], c, t));
         }
         if (MASK || j0 + 32 > keys || (p.causal && i0 < wfull)) {
           const uint8_t* mcol = MASK ? p.mask + b * p.mb + head * p.mh + (long)j * p.mj + (long)(i0 + h4) * p.mi : nullptr;
