@@ -98,7 +98,7 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
   const long base = (long)s->B * s->Hk * pl->chunks;
   long want = (512 + base - 1) / base;
-  const long most = (s->Lk + 255) / 256;
+  const long most = (s->Lk + 511) / 512;
   if (want > most) want = most;
   pl->splits = (int)(want < 1 ? 1 : want);
   if (base * pl->splits > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;

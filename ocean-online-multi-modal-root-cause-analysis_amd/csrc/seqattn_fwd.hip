@@ -171,7 +171,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 // A block's 32 rows are (query, head of the group) pairs of one key head, so a single token's G heads read the keys once; its
 // four waves take 32-key tiles in turn, each through LDS of its own, and the blocks of one row chunk split the keys further.
 // Bound by reading the keys and values once.
-template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256) void fwd_split_kernel(const Params p) {
+template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void fwd_split_kernel(const Params p) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
