@@ -16,7 +16,52 @@ from typing import Any, Dict
 import torch
 import torch.nn as nn
 
-from ... import _hip
+from ... import _hip, ops
+
+
+def _no_dropout(module: nn.Module, *drops: nn.Dropout) -> None:
+    if module.training and any(d.p > 0 for d in drops):
+        raise NotImplementedError("need_weights=False has no dropout: set it to 0 or call the module in eval mode")
+
+
+def _allowed(mask, device, four: bool):
+    """A module's mask (0 = masked, any type) as ops.attention takes it, [batch, heads, queries, keys]."""
+    if mask is None:
+        return None
+    m = torch.as_tensor(mask, device=device) != 0
+    return m if four or m.dim() < 3 else m.unsqueeze(1)
+
+
+class _Linear(torch.autograd.Function):
+    """x W^T + b (then ReLU) for rows of any number of leading dimensions, through the library's GEMMs."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, relu):
+        N, K = w.shape
+        x2 = x.contiguous().float().view(-1, K)
+        y = torch.empty(x2.shape[0], N, device=x.device, dtype=torch.float32)
+        if x2.shape[0]:
+            _hip.gemm(x2, w, y, x2.shape[0], N, K, bias=b, relu=relu)
+        ctx.save_for_backward(x2, w, y if relu else None)
+        ctx.has_bias, ctx.shape = b is not None, x.shape
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, w, y = ctx.saved_tensors
+        N, K = w.shape
+        dy = dy.contiguous().float().view(-1, N)
+        if y is not None:
+            dy = dy * (y > 0)
+        dw, db = torch.zeros_like(w), (torch.zeros(N, device=w.device) if ctx.has_bias else None)
+        dx = torch.empty_like(x2)
+        if x2.shape[0]:
+            _hip.linear_bwd(x2, dy, w, dw, db, dx, x2.shape[0], N, K)
+        return dx.view(ctx.shape), dw, db, None
+
+
+def _linear(layer: nn.Linear, x: torch.Tensor, relu: bool = False) -> torch.Tensor:
+    return _Linear.apply(x, layer.weight, layer.bias, relu)
 
 
 class ScaledDotProductAttention(nn.Module):
@@ -25,10 +70,23 @@ class ScaledDotProductAttention(nn.Module):
         self.d_model = d_model
         self.dropout = nn.Dropout(dropout)
 
-    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask=None):
+    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask=None, need_weights: bool = True, **attention):
         """The attention alone (multi_factor_attention.py:34-65): softmax(Q K^T / sqrt(d_model)) V with dropout on the
         weights, for [batch, seq_len, d] or [batch, heads, seq_len, d] inputs; mask broadcastable to the scores,
-        0 = masked.  Returns (attended values, attention weights) in the inputs' layout."""
+        0 = masked.  Returns (attended values, attention weights) in the inputs' layout.
+
+        need_weights=False: (attended values, None) through ops.attention, which stores no weights and takes any lengths, keys
+        of another length or fewer heads, fp32 or bf16, and its keyword arguments (key_lengths, causal, query_start,
+        position_table, ..).  Without dropout; a query whose mask leaves nothing gets zeros there, where the other form
+        (its masked scores are -1e9, as in the reference) gives it the mean of all values."""
+        if not need_weights:
+            _no_dropout(self, self.dropout)
+            four = query.dim() == 4
+            q, k, v = (t if four else t.unsqueeze(1) for t in (query, key, value))
+            out = ops.attention(q, k, v, mask=_allowed(mask, query.device, four), scale=1.0 / (self.d_model ** 0.5), **attention)
+            return (out if four else out.squeeze(1)), None
+        if attention:
+            raise ValueError(f"{', '.join(sorted(attention))}: only with need_weights=False")
         if query.dim() not in (3, 4) or key.shape != query.shape or value.shape != query.shape:
             raise RuntimeError(f"query, key and value of one shape [batch, (heads,) seq_len, d] expected, got "
                                f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
@@ -129,10 +187,26 @@ class MultiHeadAttention(nn.Module):
         self.attention = ScaledDotProductAttention(self.d_k, dropout)
         self.dropout = nn.Dropout(dropout)
 
-    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask=None):
+    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask=None, need_weights: bool = True, **attention):
         """The module on its own (multi_factor_attention.py:108-148): (output [B, L, D], attention weights [B, heads, L, L]
         after dropout).  As in the reference, key and value are viewed with the query's sequence length, so the three
-        must agree in shape; mask [B, L, L] (or broadcastable to it), 0 = masked."""
+        must agree in shape; mask [B, L, L] (or broadcastable to it), 0 = masked.
+
+        need_weights=False: (output, None) through ops.attention: no weights in memory, any lengths, key and value of a
+        length of their own, and its keyword arguments (key_lengths, causal, query_start, position_table, ..); see
+        ScaledDotProductAttention.forward."""
+        if not need_weights:
+            _no_dropout(self, self.dropout, self.attention.dropout)
+            if query.dim() != 3 or query.shape[2] != self.d_model or key.shape != value.shape or key.dim() != 3 or \
+                    key.shape[0] != query.shape[0] or key.shape[2] != self.d_model:
+                raise RuntimeError(f"expected query [batch, queries, {self.d_model}] and key, value [batch, keys, {self.d_model}], got "
+                                   f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
+            split = lambda t: t.view(t.shape[0], t.shape[1], self.num_heads, self.d_k).transpose(1, 2)
+            q, k, v = split(_linear(self.w_q, query)), split(_linear(self.w_k, key)), split(_linear(self.w_v, value))
+            out = ops.attention(q, k, v, mask=_allowed(mask, query.device, False), **attention)
+            return _linear(self.w_o, out.transpose(1, 2).reshape(query.shape)), None
+        if attention:
+            raise ValueError(f"{', '.join(sorted(attention))}: only with need_weights=False")
         if query.dim() != 3 or query.shape[2] != self.d_model:
             raise RuntimeError(f"expected query of shape [batch, seq_len, {self.d_model}], got {tuple(query.shape)}")
         if key.shape != query.shape or value.shape != query.shape:
@@ -163,11 +237,20 @@ class CrossModalAttention(nn.Module):
                                           nn.Linear(d_model * 4, d_model), nn.Dropout(dropout))
         self.ff_layer_norm = nn.LayerNorm(d_model)
 
-    def forward(self, query_modality: torch.Tensor, key_value_modality: torch.Tensor, mask=None):
+    def forward(self, query_modality: torch.Tensor, key_value_modality: torch.Tensor, mask=None, need_weights: bool = True, **attention):
         """The block on its own (multi_factor_attention.py:190-215): attention of the query modality over the other one,
-        residual + LayerNorm, feed-forward, residual + LayerNorm.  Returns (output, attention weights)."""
-        attended, weights = self.multihead_attention(query_modality, key_value_modality, key_value_modality, mask)
+        residual + LayerNorm, feed-forward, residual + LayerNorm.  Returns (output, attention weights).
+
+        need_weights=False: (output, None), MultiHeadAttention.forward's form of that name with its keyword arguments, and any
+        width (the driver of the other form ends at 1024)."""
+        attended, weights = self.multihead_attention(query_modality, key_value_modality, key_value_modality, mask, need_weights, **attention)
         ff = self.feed_forward
+        if not need_weights and self.d_model > 1024:
+            _no_dropout(self, ff[2], ff[4])
+            n1, n2 = self.layer_norm, self.ff_layer_norm
+            y1, _ = ops.add_layer_norm(query_modality.float(), attended, n1.weight, n1.bias, n1.eps)
+            out, _ = ops.add_layer_norm(y1, _linear(ff[3], _linear(ff[0], y1, relu=True)), n2.weight, n2.bias, n2.eps)
+            return out, weights
         drops = {m.p for m in ff if isinstance(m, nn.Dropout)}
         if len(drops) > 1 or self.layer_norm.eps != self.ff_layer_norm.eps:
             raise NotImplementedError("one dropout probability and one epsilon per block")
