@@ -122,7 +122,8 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const long key_steps = (s->Lk + key_step - 1) / key_step, query_steps = (long)G * ((s->Lq + query_step - 1) / query_step);
   plan_pieces(blocks, key_steps, s->causal, 512.0, (b16 ? 2.7 : 9.0) * wide, 128.0 * pl->D * 4, &pl->parts, &pl->part_tiles);
   plan_pieces(blocks, key_steps, s->causal, slots, (b16 ? 3.6 : 13.0 * slots / 512.0) * wide, 128.0 * pl->D * 4, &pl->dq_parts, &pl->dq_part_tiles);
-  plan_pieces((long)s->B * s->Hk * ((s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile), query_steps, s->causal, slots,
+  const long tiles_of_keys = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;      // in pairs of equal work with `causal`
+  plan_pieces((long)s->B * s->Hk * (s->causal ? (tiles_of_keys + 1) / 2 : tiles_of_keys), query_steps, false, slots,
               (b16 ? 2.9 * query_step / 32.0 : 17.0 * slots / 512.0) * wide, 128.0 * pl->D * 8, &pl->segs, &pl->seg_tiles);
   if (!pl->split && pl->parts > 1) {
     pl->ml_at = pl->fwd_floats + (size_t)blocks * pl->parts * 128 * pl->D;

@@ -255,6 +255,30 @@ template <int BM> __device__ __forceinline__ void query_tiles(const Params& p, i
   *tiles = first < p.Lq ? (p.Lq + BM - 1) / BM - *t0 : 0;
 }
 
+// What segment `seg` does of a key tile's list of query tiles (of all heads that share the key head): places u0..u1 - 1 of `all`; the
+// list is in `pieces` segments, from first_seg on.  Without `causal` a segment is seg_tiles places.  With it a tile's list is
+// shorter the later the tile, so tile t shares segments with tile k_tiles - 1 - t: the two lists behind one another, of about
+// the same length for every pair, are cut into `segs` equal segments.
+struct Span { int t0, tiles, all, u0, u1, first_seg, pieces; };
+template <int BM> __device__ __forceinline__ Span span_of(const Params& p, int tile, int seg, int keys, int start) {
+  Span s;
+  query_tiles<BM>(p, tile, keys, start, &s.t0, &s.tiles);
+  s.all = s.tiles * p.G;
+  int per = p.seg_tiles, before = 0;
+  if (p.causal) {
+    const int other = p.k_tiles - 1 - tile;
+    int t0, tiles = 0;
+    if (other != tile) query_tiles<BM>(p, other, keys, start, &t0, &tiles);
+    per = max(1, (s.all + tiles * p.G + p.segs - 1) / p.segs);
+    if (tile > other) before = tiles * p.G;
+  }
+  s.u0 = min(max(seg * per - before, 0), s.all);
+  s.u1 = min(max((seg + 1) * per - before, 0), s.all);
+  s.first_seg = min(before / per, p.segs - 1);
+  s.pieces = s.all > 0 ? (before + s.all - 1) / per - s.first_seg + 1 : 0;
+  return s;
+}
+
 // A wave keeps its 32 keys' dk and dv in registers, and the keys as right operand; the values too where that leaves room for two
 // waves on a SIMD, else they stay in LDS (VL): at 128 16-bit features the registers of both were 440, and half of the instructions
 // moved accumulators between the two register files.
@@ -281,32 +305,50 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     diag.below = diag.above = 0.f;
     if (sum_bias) for (int x = tid; x < 4 * slots; x += 256) dist_sums[x] = 0.f;
   }
-  // a key head's list: the first segment of every key tile, then the second, ..; with `causal` the first tiles have the most queries
+  // With `causal` a pair's segment lies in one tile or in the end of one and the beginning of the other: blocks for the longer part
+  // of every segment come first, blocks for the rest fill the places that those with a rest leave early.
   const int k_tiles = p.k_tiles;
   int bk, place;
-  work_of(p, blockIdx.x, gridDim.x, k_tiles * p.segs, &bk, &place);
-  const int tile = place % k_tiles, seg = place / k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
-  const int keys = keys_of(p, b), start = start_of(p, b);
+  work_of(p, blockIdx.x, gridDim.x, p.causal ? (k_tiles + 1) / 2 * 2 * p.segs : k_tiles * p.segs, &bk, &place);
+  const int b = bk / p.Hk, kh = bk % p.Hk, head0 = kh * p.G, keys = keys_of(p, b), start = start_of(p, b);
+  int tile = place % k_tiles, seg = place / k_tiles;
+  Span span;
+  if (p.causal) {
+    const int pairs = (k_tiles + 1) / 2, second = place / (pairs * p.segs), r = place % (pairs * p.segs);
+    seg = r / pairs;
+    const int t1 = r % pairs, t2 = k_tiles - 1 - t1;
+    if (t1 == t2 && second) return;
+    const Span s1 = span_of<BM>(p, t1, seg, keys, start), s2 = span_of<BM>(p, t2, seg, keys, start);
+    const bool take2 = t1 != t2 && (s2.u1 - s2.u0 > s1.u1 - s1.u0) != (second != 0);
+    tile = take2 ? t2 : t1;
+    span = take2 ? s2 : s1;
+  } else {
+    span = span_of<BM>(p, tile, seg, keys, start);
+  }
+  const int u0 = span.u0, u1 = span.u1, tiles = span.tiles, t0 = span.t0;
+  if (sum_bias) {                                           // the heads that this segment does not reach
+    const int g0 = u0 < u1 ? u0 / tiles : 0, g1 = u0 < u1 ? (u1 - 1) / tiles : -1;
+    for (int x = tid; x < p.G * p.buckets; x += 256) {
+      const int g = x / p.buckets;
+      if (g < g0 || g > g1) p.dtable_part[((((long)(head0 + g) * p.B + b) * k_tiles + tile) * p.segs + seg) * p.buckets + x % p.buckets] = 0.f;
+    }
+  }
+  if (u0 >= u1 && (span.all > 0 || seg != span.first_seg)) return;
+  const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
+  const float c = p.scale * kLog2e, row_unit = 1.f / c;
+  const Async<T, D, BM, 256> qload(p.q.l, tid), gload(p.go.l, tid);
   const int j0 = tile * kRows + 32 * w, j = j0 + (lane & 31);
   const bool live = j < keys;
   RowRegs<T, D> k, v;
   k.load(live ? (const T*)p.k.p + b * p.k.b + kh * p.k.h + (long)j * p.k.l : nullptr, p.d, lane);
-  const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
   if (!VL) v.load(live ? vb + (long)j * p.v.l : nullptr, p.d, lane);
-  const float c = p.scale * kLog2e;
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) { dk[db] = f32x16{}; dv[db] = f32x16{}; }
   // queries from wfirst on see some key of this wave; from wfull on every key
   int wfirst = 0, wfull = 0;
   if (p.causal) { wfirst = max(j0 - start, 0); wfull = j0 + 31 - start; }
-  int t0, tiles;
-  query_tiles<BM>(p, tile, keys, start, &t0, &tiles);
-  const int all = tiles * p.G, u0 = min(seg * p.seg_tiles, all), u1 = min(u0 + p.seg_tiles, all);
-  const int head0 = kh * p.G;
-  const Async<T, D, BM, 256> qload(p.q.l, tid), gload(p.go.l, tid);
   float rv = 0.f;                                           // threads 0..BM-1: -lse, BM..2BM-1: -delta
-  const float row_unit = 1.f / c;
   const auto load = [&](int u, int buf) {
     const int head = head0 + u / tiles, r0 = (t0 + u % tiles) * BM;
     if (tid < 2 * BM) {
@@ -395,15 +437,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     if (sum_bias && (u == u1 - 1 || u % tiles == tiles - 1))
       store_bias_sums(p, diag, dist_sums, p.dtable_part + ((((long)head * p.B + b) * k_tiles + tile) * p.segs + seg) * p.buckets, tid);
   }
-  if (sum_bias) {                                           // the heads that this segment does not reach
-    const int g0 = u0 < u1 ? u0 / tiles : 0, g1 = u0 < u1 ? (u1 - 1) / tiles : -1;
-    for (int x = tid; x < p.G * p.buckets; x += 256) {
-      const int g = x / p.buckets;
-      if (g < g0 || g > g1) p.dtable_part[((((long)(head0 + g) * p.B + b) * k_tiles + tile) * p.segs + seg) * p.buckets + x % p.buckets] = 0.f;
-    }
-  }
-  if (seg > 0 && u0 >= u1) return;
-  if (all > p.seg_tiles) {                                  // more than one segment: sums in the matrix instructions' layout
+  if (span.pieces > 1) {                                    // sums in the matrix instructions' layout
     float* part = p.part_o + ((((long)bk * k_tiles + tile) * p.segs + seg) * 4 + w) * (2 * 32 * D);
     store_part<D>(part, dk, lane);
     store_part<D>(part + 32 * D, dv, lane);
@@ -443,15 +477,13 @@ template <typename T, int D> __global__ __launch_bounds__(256) void dkv_join_ker
   constexpr int BM = BwdTile<T, D>::kRows, kPieces = D / 8;  // 16-byte pieces a lane: D / 32 blocks x 4, of dk and of dv
   const int unit = blockIdx.x >> 2, w = blockIdx.x & 3, lane = threadIdx.x & 63;
   const int tile = unit % p.k_tiles, bk = unit / p.k_tiles, b = bk / p.Hk, kh = bk % p.Hk;
-  int t0, tiles;
-  query_tiles<BM>(p, tile, keys_of(p, b), start_of(p, b), &t0, &tiles);
-  const int all = tiles * p.G;
-  if (all <= p.seg_tiles) return;
-  const int segs = (all + p.seg_tiles - 1) / p.seg_tiles, j = tile * kRows + 32 * w + (lane & 31);
-  const float* part = p.part_o + ((long)unit * p.segs * 4 + w) * (2 * 32 * D) + lane * 4;
+  const Span span = span_of<BM>(p, tile, 0, keys_of(p, b), start_of(p, b));
+  if (span.pieces <= 1) return;
+  const int j = tile * kRows + 32 * w + (lane & 31);
+  const float* part = p.part_o + (((long)unit * p.segs + span.first_seg) * 4 + w) * (2 * 32 * D) + lane * 4;
   for (int n = threadIdx.x >> 6; n < 2 * kPieces; n += 4) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < segs; ++s) t += *reinterpret_cast<const f32x4*>(part + (long)s * 4 * (2 * 32 * D) + n * 256);
+    for (int s = 0; s < span.pieces; ++s) t += *reinterpret_cast<const f32x4*>(part + (long)s * 4 * (2 * 32 * D) + n * 256);
     const bool value = n >= kPieces;
     const View& o = value ? p.dv : p.dk;
     const float f = value ? 1.f : p.scale;
@@ -498,8 +530,8 @@ template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p,
     lds = (4 * BM + (values_in_lds(D * sizeof(T)) ? kRows : 0)) * TL::kRowBytes + 4 * BM * sizeof(float) + (BIAS ? slots * sizeof(float) : 0);
     if (BIAS && p.dtable_part) lds += 4 * slots * sizeof(float);
     OCEAN_TRY(set_lds(dkv_kernel<T, D, BIAS, MASK>, lds));
-    const long units = (long)p.B * p.Hk * p.k_tiles;
-    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)(units * p.segs)), dim3(256), lds, s, p);
+    const long units = (long)p.B * p.Hk * p.k_tiles, blocks = (long)p.B * p.Hk * (p.causal ? (p.k_tiles + 1) / 2 * 2 : p.k_tiles) * p.segs;
+    hipLaunchKernelGGL((dkv_kernel<T, D, BIAS, MASK>), dim3((unsigned)blocks), dim3(256), lds, s, p);
     OCEAN_LAUNCH_CHECK();
     if (p.segs > 1 && (p.dk.p || p.dv.p)) {
       hipLaunchKernelGGL((dkv_join_kernel<T, D>), dim3((unsigned)(units * 4)), dim3(256), 0, s, p);
