@@ -566,7 +566,8 @@ int ocean_clip_adam_step_auto(const ocean_adam_chunk* table, int n_chunks, ocean
  * [B, H, L, L].  out_i = sum_j p_ij v_j with p_i = softmax over the allowed keys j of scale * q_i . k_j (+ position bias); a
  * query with no allowed key gets zeros.  Query i of sample b stands at position starts[b] + i (query_start + i without
  * `starts`) among the keys.  Allowed: j < lengths[b] (clamped to 0..Lk; NULL: Lk), with causal j <= the query's position, and
- * with a mask mask[b, h, i, j] != 0.  Keys and values past a sample's length are not read.  Query head h reads key head
+ * with a mask mask[b, h, i, j] != 0.  Keys and values past a sample's length are not read, nor are those that a mask of query
+ * stride 0 (and head stride 0 when key heads are shared) takes, nor queries that one of key stride 0 takes.  Query head h reads key head
  * h / (H / Hk).  Positions are int32, |position| < 2^30.
  * Position bias: table[bucket(j - position)][h] is added to the score.  With side = num_buckets (bidirectional: half of them for
  * each sign, the upper half for keys after the query) and E = side / 2, distances n < E have a bucket each, farther ones share

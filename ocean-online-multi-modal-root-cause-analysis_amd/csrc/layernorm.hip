@@ -365,7 +365,7 @@ int bwd_blocks(long rows, int W, int type) {
   const int E = type == OCEAN_F32 ? 4 : 8;
   const long chunks = (W + E - 1) / E;
   const long groups = chunks <= 8 ? 32 : chunks <= 16 ? 16 : chunks <= 32 ? 8 : chunks <= 128 ? 4 : 1;   // rows of a block at a time
-  const long most = chunks <= 512 ? 768 : chunks <= 1024 ? 512 : 256;
+  const long fit = (1L << 24) / W, most = chunks <= 512 ? 768 : chunks <= 1024 ? 512 : fit > 256 ? 256 : fit > 16 ? fit : 16;
   const long sets = (rows + groups - 1) / groups, per = (sets + most - 1) / most;
   return (int)((sets + per - 1) / per);
 }

@@ -133,6 +133,14 @@ template <int D> __device__ __forceinline__ f32x16 col_mma(const char* t, int ro
   return acc;
 }
 
+// Rows that a mask takes from everything: a key that no query of the sample and head sees (a mask without a query axis), a query
+// that sees no key (one without a key axis).  They are not read, so whatever padding they hold reaches no sum.
+struct Keep {
+  const uint8_t* at = nullptr;
+  long step = 0;
+  __device__ __forceinline__ bool has(int row) const { return at == nullptr || at[(long)row * step] != 0; }
+};
+
 // ---------------------------------------------------------------- global memory, any alignment
 // 16 bytes of a row of d features from feature e0 on; features past d are zero, memory past the row is not touched.
 // A row's last, partial chunk is read as the 16 bytes that end with the row, shifted into place (d >= one chunk).
@@ -158,13 +166,13 @@ template <typename T, int D, int ROWS, int THREADS> struct Stage {
   typedef Tile<T, D> TL;
   static constexpr int kN = (ROWS * TL::kCh + THREADS - 1) / THREADS;
   u32x4 r[kN];
-  // rows row0.. of a sequence; rows from `rows` on are zero and not read
-  __device__ __forceinline__ void fetch(const T* base, long stride, int row0, int rows, int d, int tid) {
+  // rows row0.. of a sequence; rows from `rows` on, and those that `keep` leaves out, are zero and not read
+  __device__ __forceinline__ void fetch(const T* base, long stride, int row0, int rows, int d, int tid, Keep keep = Keep{}) {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       const int id = tid + n * THREADS, row = id / TL::kCh, c = id % TL::kCh;
       u32x4 x = {0u, 0u, 0u, 0u};
-      if (row < ROWS && row0 + row < rows) x = load_chunk<T>(base + (long)(row0 + row) * stride, c * Mm<T>::kEpc, d);
+      if (row < ROWS && row0 + row < rows && keep.has(row0 + row)) x = load_chunk<T>(base + (long)(row0 + row) * stride, c * Mm<T>::kEpc, d);
       r[n] = x;
     }
   }
@@ -195,10 +203,10 @@ template <typename T, int D, int ROWS, int THREADS> struct Async {
       off[n] = (long)row * stride + ((id % TL::kCh) ^ TL::swz(row)) * E;
     }
   }
-  __device__ __forceinline__ void load(char* t, const T* base, long stride, int row0, int rows, int d, int tid) const {
+  __device__ __forceinline__ void load(char* t, const T* base, long stride, int row0, int rows, int d, int tid, Keep keep = Keep{}) const {
     char* const to = t + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
     const T* const first = base + (long)row0 * stride;
-    if (row0 + ROWS <= rows && d == D) {
+    if (row0 + ROWS <= rows && d == D && keep.at == nullptr) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) issue(kEven ? first + (long)n * kStep * stride + off[0] : first + off[kEven ? 0 : n], to + n * THREADS * 16);
     } else {
@@ -206,7 +214,7 @@ template <typename T, int D, int ROWS, int THREADS> struct Async {
       for (int n = 0; n < kN; ++n) {
         const int id = tid + n * THREADS, row = id / TL::kCh, c = (id % TL::kCh) ^ TL::swz(row);
         const T* from = kEven ? first + (long)n * kStep * stride + off[0] : first + off[kEven ? 0 : n];
-        if (row0 + row >= rows || c * E >= d) from = reinterpret_cast<const T*>(kZeros);
+        if (row0 + row >= rows || c * E >= d || !keep.has(row0 + row)) from = reinterpret_cast<const T*>(kZeros);
         issue(from, to + n * THREADS * 16);
       }
     }
@@ -269,6 +277,13 @@ __device__ __forceinline__ float other_half_sum(float x) {
 // ---------------------------------------------------------------- places
 __device__ __forceinline__ int keys_of(const Params& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk; }
 __device__ __forceinline__ int start_of(const Params& p, int b) { return p.starts ? min(max(p.starts[b], -(1 << 30)), 1 << 30) : p.start0; }
+
+__device__ __forceinline__ Keep kept_keys(const Params& p, int b, int head) {
+  return p.mask && p.mi == 0 ? Keep{p.mask + b * p.mb + head * p.mh, p.mj} : Keep{};
+}
+__device__ __forceinline__ Keep kept_queries(const Params& p, int b, int head) {
+  return p.mask && p.mj == 0 ? Keep{p.mask + b * p.mb + head * p.mh, p.mi} : Keep{};
+}
 
 // bit e: mask[.., j + e] allows (row: the mask's row of this query; j + e < keys)
 __device__ __forceinline__ uint32_t mask4(const Params& p, const uint8_t* row, int j, int keys) {

@@ -140,9 +140,12 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   if (part > 0 && u0 >= u1) return;
   const T* kb = (const T*)p.k.p + b * p.k.b + kh * p.k.h;
   const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
+  Keep kk;
+  bool own = live;
+  if (MASK) { kk = kept_keys(p, b, head); own = live && kept_queries(p, b, head).has(i); }
   RowRegs<T, D> q, go;
-  q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
-  go.load(live ? (const T*)p.go.p + b * p.go.b + head * p.go.h + (long)i * p.go.l : nullptr, p.d, lane);
+  q.load(own ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
+  go.load(own ? (const T*)p.go.p + b * p.go.b + head * p.go.h + (long)i * p.go.l : nullptr, p.d, lane);
   float delta = 0.f, lse = INFINITY;
   if (live) {
     RowRegs<T, D> o;
@@ -164,16 +167,16 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
   const Async<T, D, BN, 256> kload(p.k.l, tid), vload(p.v.l, tid);
   if (u0 < u1) {
-    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
-    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
+    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid, kk);
+    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid, kk);
   }
   // Up to two tiles of keys sit in the two buffers.  Rows of so few keys are where 16-bit rounding of `o` reaches dq through delta
   // (its share shrinks with the root of the number of keys that carry weight): their delta is formed from p and dp first
   // (a part has two tiles at least, so they are never split).
   const bool few = sizeof(T) == 2 && tiles <= 2;
   if (few && tiles == 2) {
-    kload.load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid);
-    vload.load(vt + kBuf, vb, p.v.l, BN, keys, p.d, tid);
+    kload.load(kt + kBuf, kb, p.k.l, BN, keys, p.d, tid, kk);
+    vload.load(vt + kBuf, vb, p.v.l, BN, keys, p.d, tid, kk);
   }
   if (few) {
     wait_tiles();
@@ -195,8 +198,8 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       wait_tiles();
       __syncthreads();
       if (t + 1 < u1) {
-        kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
-        vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
+        kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid, kk);
+        vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid, kk);
       }
     }
     if (j0 < wend) {
@@ -338,7 +341,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   const float c = p.scale * kLog2e, row_unit = 1.f / c;
   const Async<T, D, BM, 256> qload(p.q.l, tid), gload(p.go.l, tid);
   const int j0 = tile * kRows + 32 * w, j = j0 + (lane & 31);
-  const bool live = j < keys;
+  Keep kk;                                                  // (of all heads of the group)
+  if (MASK && (p.mh == 0 || p.G == 1)) kk = kept_keys(p, b, head0);
+  const bool live = j < keys && kk.has(j);
   RowRegs<T, D> k, v;
   k.load(live ? (const T*)p.k.p + b * p.k.b + kh * p.k.h + (long)j * p.k.l : nullptr, p.d, lane);
   if (!VL) v.load(live ? vb + (long)j * p.v.l : nullptr, p.d, lane);
@@ -351,17 +356,19 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   float rv = 0.f;                                           // threads 0..BM-1: -lse, BM..2BM-1: -delta
   const auto load = [&](int u, int buf) {
     const int head = head0 + u / tiles, r0 = (t0 + u % tiles) * BM;
+    Keep kq;
+    if (MASK) kq = kept_queries(p, b, head);
     if (tid < 2 * BM) {
       const int i = r0 + tid % BM;
       const float* from = tid < BM ? p.lse : p.delta;
       rv = i < p.Lq ? -from[((long)b * p.H + head) * p.Lq + i] : tid < BM ? -INFINITY : 0.f;
       if (FROM_LSE && tid < BM) rv *= row_unit;
     }
-    qload.load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid);
-    gload.load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid);
+    qload.load(qt + buf * kBuf, (const T*)p.q.p + b * p.q.b + head * p.q.h, p.q.l, r0, p.Lq, p.d, tid, kq);
+    gload.load(gt + buf * kBuf, (const T*)p.go.p + b * p.go.b + head * p.go.h, p.go.l, r0, p.Lq, p.d, tid, kq);
   };
   if (u0 < u1) {
-    if (VL) Async<T, D, kRows, 256>(p.v.l, tid).load(vt, vb, p.v.l, tile * kRows, keys, p.d, tid);
+    if (VL) Async<T, D, kRows, 256>(p.v.l, tid).load(vt, vb, p.v.l, tile * kRows, keys, p.d, tid, kk);
     load(u0, u0 & 1);
     if (BIAS) fill_bias(p, head0 + u0 / tiles, lut, tid, 256);
   }

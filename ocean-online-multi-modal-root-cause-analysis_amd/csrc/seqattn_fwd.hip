@@ -102,8 +102,11 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   const T* kb = (const T*)p.k.p + b * p.k.b + kh * p.k.h;
   const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
   const bool live = i < p.Lq;
+  Keep kk;
+  bool own = live;
+  if (MASK) { kk = kept_keys(p, b, head); own = live && kept_queries(p, b, head).has(i); }
   RowRegs<T, D> q;
-  q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
+  q.load(own ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
   const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
   const int tiles = key_tiles<BN>(p, tile, keys, start), u0 = part * p.part_tiles, u1 = min(u0 + p.part_tiles, tiles);
   if (part > 0 && u0 >= u1) return;
@@ -117,16 +120,16 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
   const Async<T, D, BN, 256> kload(p.k.l, tid), vload(p.v.l, tid);
   if (u0 < u1) {
-    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid);
-    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid);
+    kload.load(kt + (u0 & 1) * kBuf, kb, p.k.l, u0 * BN, keys, p.d, tid, kk);
+    vload.load(vt + (u0 & 1) * kBuf, vb, p.v.l, u0 * BN, keys, p.d, tid, kk);
   }
   for (int t = u0; t < u1; ++t) {
     const int j0 = t * BN, cur = t & 1;
     wait_tiles();
     __syncthreads();
     if (t + 1 < u1) {
-      kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid);
-      vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid);
+      kload.load(kt + (cur ^ 1) * kBuf, kb, p.k.l, j0 + BN, keys, p.d, tid, kk);
+      vload.load(vt + (cur ^ 1) * kBuf, vb, p.v.l, j0 + BN, keys, p.d, tid, kk);
     }
     if (j0 < wend) {
       f32x16 s[NS];
@@ -189,8 +192,14 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   }
   const T* kb = (const T*)p.k.p + b * p.k.b + kh * p.k.h;
   const T* vb = (const T*)p.v.p + b * p.v.b + kh * p.v.h;
+  Keep kk;                                                  // (of all heads of the group)
+  bool own = live;
+  if (MASK) {
+    if (p.mh == 0 || p.G == 1) kk = kept_keys(p, b, kh * p.G);
+    own = live && kept_queries(p, b, head).has(i);
+  }
   RowRegs<T, D> q;
-  q.load(live ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
+  q.load(own ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
   const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
   const int last = start + min((chunk * 32 + 31) / p.G, p.Lq - 1);
   const int end = p.causal ? min(keys, last + 1) : keys;
@@ -205,15 +214,15 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   Stage<T, D, 32, 64> ks, vs;
   int t = split * per + w;
   if (t < t1) {
-    ks.fetch(kb, p.k.l, 32 * t, keys, p.d, lane);
-    vs.fetch(vb, p.v.l, 32 * t, keys, p.d, lane);
+    ks.fetch(kb, p.k.l, 32 * t, keys, p.d, lane, kk);
+    vs.fetch(vb, p.v.l, 32 * t, keys, p.d, lane, kk);
   }
   for (; t < t1; t += 4) {
     ks.put(kt, lane);
     vs.put(vt, lane);
     if (t + 4 < t1) {
-      ks.fetch(kb, p.k.l, 32 * (t + 4), keys, p.d, lane);
-      vs.fetch(vb, p.v.l, 32 * (t + 4), keys, p.d, lane);
+      ks.fetch(kb, p.k.l, 32 * (t + 4), keys, p.d, lane, kk);
+      vs.fetch(vb, p.v.l, 32 * (t + 4), keys, p.d, lane, kk);
     }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();

@@ -508,9 +508,11 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
     product in the inputs' type.
 
     mask: bool or uint8, broadcastable to [batch, heads, queries, keys], nonzero = allowed.  key_lengths: int32 [batch] on the
-    GPU, each sample's key count (clamped to 0..keys); what lies behind is never read, its gradient is zero.  A place that a
-    mask or `causal` takes from some queries only still enters their sums with weight zero, so it has to be finite.  A query
-    with no allowed key gets zeros, and passes no gradient.
+    GPU, each sample's key count (clamped to 0..keys); what lies behind is never read, its gradient is zero.  The same holds for
+    keys that a mask without a query axis takes (size 1 there; with shared key heads without a head axis too), and for queries
+    that one without a key axis takes.  Any other place that a mask or `causal` takes away still enters sums, with weight zero:
+    its key, value, query and the gradient that arrives have to be finite.  A query with no allowed key gets zeros, and passes
+    no gradient.
     query_start: position of the first query among the keys, an int or int32 [batch] on the GPU; default keys - queries (the
     queries are the last keys).  It places `causal` (keys up to the query's own position) and the position bias.
     position_table [buckets, heads]: the learned bias of the distance key - query position, added to the scaled scores.

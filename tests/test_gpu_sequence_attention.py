@@ -200,6 +200,42 @@ def test_what_lies_behind_a_sample_is_not_read(dtype, Lq):
         assert torch.equal(x, y) and torch.isfinite(x).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Lq", [2, 140])
+def test_what_a_padding_mask_takes_is_not_read(dtype, Lq):
+    """NaN and infinities in keys and values that a mask [batch, 1, 1, keys] takes, in queries and in the arriving gradient where one
+    of [batch, 1, queries, 1] does."""
+    from ocean import ops
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v, w = (heads_view(3, 4 if s in (1, 4) else 2, Lq if s in (1, 4) else 130, 64, dtype, s).detach() for s in (1, 2, 3, 4))
+    by_key = torch.rand(3, 1, 1, 130, device="cuda", generator=g) < 0.7
+    by_query = torch.rand(3, 1, Lq, 1, device="cuda", generator=g) < 0.5
+    for mask, dirty in ((by_key, (1, 2)), (by_query, (0, 3))):
+        sets = []
+        for spoil in (False, True):
+            t = [x.clone() for x in (q, k, v, w)]
+            if spoil:
+                gone = ~(mask.transpose(2, 3) if dirty[0] else mask)
+                for n, fill in zip(dirty, (float("nan"), float("-inf"))):
+                    t[n] = t[n].masked_fill(gone, fill)
+            leaves = [x.requires_grad_(True) for x in t[:3]]
+            out = ops.attention(*leaves, mask=mask)
+            sets.append([out, *torch.autograd.grad(out, leaves, t[3])])
+            assert torch.equal(out, ops.attention(*(x.detach() for x in leaves), mask=mask))
+        for a, b in zip(*sets):
+            assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    from ocean import ops
+    q = torch.randn(1, 1, 4, 16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiated"):
+        torch.autograd.grad(ops.attention(q, q, q).sum(), q, create_graph=True)
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiated"):
+        torch.autograd.grad(ops.layer_norm(x).sum(), x, create_graph=True)
+
+
 def test_nothing_to_attend_to():
     from ocean import ops
     for Lq, Lk, B in ((3, 0, 2), (0, 5, 2), (3, 5, 0)):
