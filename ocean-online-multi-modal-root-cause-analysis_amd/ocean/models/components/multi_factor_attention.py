@@ -41,13 +41,15 @@ class _Linear(torch.autograd.Function):
         x2 = x.contiguous().float().view(-1, K)
         y = torch.empty(x2.shape[0], N, device=x.device, dtype=torch.float32)
         if x2.shape[0]:
-            _hip.gemm(x2, w, y, x2.shape[0], N, K, bias=b, relu=relu)
+            with torch.cuda.device_of(x2):
+                _hip.gemm(x2, w, y, x2.shape[0], N, K, bias=b, relu=relu)
         ctx.save_for_backward(x2, w, y if relu else None)
         ctx.has_bias, ctx.shape = b is not None, x.shape
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
     def backward(ctx, dy):
+        ops._once()
         x2, w, y = ctx.saved_tensors
         N, K = w.shape
         dy = dy.contiguous().float().view(-1, N)
@@ -56,7 +58,8 @@ class _Linear(torch.autograd.Function):
         dw, db = torch.zeros_like(w), (torch.zeros(N, device=w.device) if ctx.has_bias else None)
         dx = torch.empty_like(x2)
         if x2.shape[0]:
-            _hip.linear_bwd(x2, dy, w, dw, db, dx, x2.shape[0], N, K)
+            with torch.cuda.device_of(x2):
+                _hip.linear_bwd(x2, dy, w, dw, db, dx, x2.shape[0], N, K)
         return dx.view(ctx.shape), dw, db, None
 
 

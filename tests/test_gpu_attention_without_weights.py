@@ -129,3 +129,14 @@ def test_refusals():
         CrossModalAttention(32, 4, 0.1).cuda().train()(x, x, need_weights=False)
     with pytest.raises(RuntimeError):
         MultiHeadAttention(32, 4).cuda().eval()(x, x[:1], x[:1], need_weights=False)
+
+
+def test_second_derivatives_are_refused():
+    from ocean.models.components import MultiHeadAttention
+    m = MultiHeadAttention(32, 2, dropout=0.0).cuda()
+    x = torch.randn(1, 5, 32, device="cuda")
+    for p in m.parameters():
+        p.requires_grad_(False)
+    m.w_o.weight.requires_grad_(True)                       # its projection alone is on the way back
+    with pytest.raises(RuntimeError, match="differentiated"):
+        torch.autograd.grad(m(x, x, x, need_weights=False)[0].square().sum(), m.w_o.weight, create_graph=True)
