@@ -86,12 +86,14 @@ class Transport:
             pg.shutdown() if hasattr(pg, "shutdown") else dist.destroy_process_group(pg)
 
     def quiesce(self) -> None:
-        """Before a step with collectives is recorded into a HIP graph: finish the device's work, so that every
-        collective of the eager steps has completed before the recording starts.  (The process group's watchdog thread
-        goes on polling the events of collectives it still lists; ocean._hip.capture records in thread-local capture
-        mode, in which the runtime refuses unsafe calls of the recording thread only, so those polls are legal.)"""
+        """Before a step with collectives is recorded into a HIP graph: finish the device's work, then wait until the
+        process group's watchdog thread has dropped every collective of the eager steps from its list.  Their events were
+        recorded on the group's own stream, which the recording captures; a poll that falls into it fails
+        (hipErrorCapturedEvent, in any capture mode) and ends the process.  Recorded collectives are not listed."""
         if self.backend == "nccl":
             torch.cuda.synchronize()
+            pg = self.group if self.group is not None else dist.distributed_c10d._get_default_group()
+            pg._wait_for_pending_works()
 
 
 class _ThenScale:
