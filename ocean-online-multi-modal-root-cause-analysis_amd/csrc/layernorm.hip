@@ -82,6 +82,7 @@ struct LnP {
 
 template <int LPR> struct Block { static constexpr int kThreads = LPR > 256 ? LPR : 256; };
 
+// 4099 rows of 8192 fp32: 52 us = 5.2 TB/s, what a large copy reaches; 16384 of 768 bf16 with a residual: 21 us (101 MB, 4.8 TB/s).
 template <typename T, int E, int LPR, int NC, bool RES> __global__ __launch_bounds__(Block<LPR>::kThreads) void fwd_kernel(const LnP p) {
   constexpr int kT = Block<LPR>::kThreads;
   __shared__ float red[LPR > 64 ? LPR / 64 : 1];
@@ -162,7 +163,7 @@ template <typename T, bool RES> __global__ __launch_bounds__(1024) void fwd_wide
 }
 
 // Rows that take a whole block: the next row is loaded before this one's sums, so that memory works while the block's waves meet
-// (4099 rows of 8192 fp32: 106 us without, 84 with).
+// (4099 rows of 8192 fp32: 106 us without, 84 with, 4.8 TB/s; 16384 of 768 bf16, one gradient more: 27 us, 3.7 TB/s).
 template <typename T, int E, int LPR, int NC> __global__ __launch_bounds__(Block<LPR>::kThreads) void bwd_kernel(const LnP p) {
   constexpr int kT = Block<LPR>::kThreads, kG = kT / LPR;
   constexpr bool kNext = LPR >= 256;

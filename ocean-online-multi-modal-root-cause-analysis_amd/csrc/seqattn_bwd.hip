@@ -120,6 +120,10 @@ template <typename T, int D> struct BwdTile {
   static constexpr int kKeys = key_tile(sizeof(T) == 2);    // keys at a time of the launch over queries
 };
 
+// Launch over queries, three products (s, dp, dq): the wave's 32 queries and their d_out in registers, keys and values through two
+// LDS buffers each.  Bound by the turns of its two waves a SIMD between matrix cores (busy 0.44 of the cycles), vector units (0.36)
+// and tiles (waiting 0.40); the registers hold no third wave and no second tile.  Causal 2 x 16
+// heads (4 of keys) x 4096 x 128 bf16: 235 us = 0.88 PFLOP/s of the three products; 8 x 8 heads x 512 x 96 fp32, ragged: 97 us.
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BN = BwdTile<T, D>::kKeys, NS = BN / 32;
@@ -284,7 +288,8 @@ template <int BM> __device__ __forceinline__ Span span_of(const Params& p, int t
 
 // A wave keeps its 32 keys' dk and dv in registers, and the keys as right operand; the values too where that leaves room for two
 // waves on a SIMD, else they stay in LDS (VL): at 128 16-bit features the registers of both were 440, and half of the instructions
-// moved accumulators between the two register files.
+// moved accumulators between the two register files.  Four products (s, dp, dv, dk).  Bound as the launch over queries is: causal
+// 2 x 16 heads (4 of keys) x 4096 x 128 bf16: 425 us = 0.65 PFLOP/s of the four; 8 x 8 heads x 512 x 96 fp32, ragged: 135 us.
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;
