@@ -148,7 +148,9 @@ int fill(const ocean_attention_shape* s, const Plan& pl, const void* q, const vo
   p.q = view(q, s->q_strides); p.k = view(k, s->k_strides); p.v = view(v, s->v_strides);
   p.B = s->B; p.H = s->H; p.Hk = s->Hk; p.G = s->H / s->Hk; p.Lq = s->Lq; p.Lk = s->Lk; p.d = s->d; p.scale = s->scale; p.causal = s->causal != 0;
   p.start0 = s->query_start; p.lengths = lengths; p.starts = starts;
-  p.mask = mask; p.mb = s->mask_strides[0]; p.mh = s->mask_strides[1]; p.mi = s->mask_strides[2]; p.mj = s->mask_strides[3];
+  p.mask = mask; p.mb = s->mask_strides[0]; p.mh = s->mask_strides[1];
+  // an axis of one place has no stride: kept_keys and kept_queries know a mask without queries or without keys by its zero there
+  p.mi = s->Lq == 1 ? 0 : s->mask_strides[2]; p.mj = s->Lk == 1 ? 0 : s->mask_strides[3];
   p.table = table; p.buckets = s->num_buckets; p.both = s->bidirectional != 0; p.max_dist = s->max_distance;
   if (table) {
     p.side = p.both ? p.buckets / 2 : p.buckets;
