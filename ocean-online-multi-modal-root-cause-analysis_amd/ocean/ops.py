@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -379,7 +380,7 @@ def diversity_loss(x: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------- sequences: attention without stored weights, layer norm
 # Small calls are bound by what the host does for them, so these two functions pack their shape structures in one step, ask
-# for the raw stream handle, and go around autograd where nothing needs a gradient.
+# for the raw stream handle, and go around autograd where nothing needs a gradient, outside traces and forward-mode levels.
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _pack_attention = struct.Struct("@9if4i28l").pack            # ocean_attention_shape
 _pack_norm = struct.Struct("@l2if4x4l").pack                 # ocean_layer_norm_shape
@@ -416,6 +417,12 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 def _once() -> None:
     if torch.is_grad_enabled():
         raise RuntimeError("the backward pass of this operator cannot itself be differentiated (create_graph=True)")
+
+
+def _through_autograd(grad: bool) -> bool:
+    """Whether a call has to go through its autograd function: for a gradient, in a trace (which records the function but would
+    miss what the library writes) and inside a forward-mode level (where the function refuses a tangent that would be lost)."""
+    return (grad and torch.is_grad_enabled()) or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
 
 
 _NO_STRIDES = (0, 0, 0)
@@ -482,7 +489,7 @@ class _Attention(torch.autograd.Function):
 
 
 def _attention(q, k, v, mask, lengths, starts, table, cfg):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+    if _through_autograd(q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
         return _Attention.apply(q, k, v, mask, lengths, starts, table, cfg)
     return _attention_forward(q, k, v, mask, lengths, starts, table, cfg, False)[0]
 
@@ -681,7 +688,7 @@ def _norm(x, residual, weight, bias, eps):
 
 
 def _norm_call(x, residual, weight, bias, eps, grad):
-    if grad and torch.is_grad_enabled():
+    if _through_autograd(grad):
         return _LayerNorm.apply(x, residual, weight, bias, eps)
     y, total = _norm_forward(x, residual, weight, bias, eps, False)[:2]
     return y if total is None else (y, total)
