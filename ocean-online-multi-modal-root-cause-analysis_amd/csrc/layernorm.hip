@@ -77,6 +77,7 @@ struct LnP {
   const float* w; const float* b;
   void* y; void* sum; float* stats;              // y, sum: dense rows
   long rows; int W; float eps;
+  long row0;                                     // forward: first row of the launch
   const void* dy; long lddy; const void* dsum; long ldds; void* dx; float* part; int blocks;
 };
 
@@ -87,7 +88,7 @@ template <typename T, int E, int LPR, int NC, bool RES> __global__ __launch_boun
   constexpr int kT = Block<LPR>::kThreads;
   __shared__ float red[LPR > 64 ? LPR / 64 : 1];
   const int lane = threadIdx.x % LPR;
-  const long row = (long)blockIdx.x * (kT / LPR) + threadIdx.x / LPR;
+  const long row = p.row0 + (long)blockIdx.x * (kT / LPR) + threadIdx.x / LPR;
   if (row >= p.rows) return;                     // LPR > 64: the block has one row (or kT == LPR rows apart), all threads agree
   float f[NC][E];
   float s[1] = {0.f};
@@ -138,7 +139,7 @@ template <typename T, int E, int LPR, int NC, bool RES> __global__ __launch_boun
 // rows wider than a block's registers: the row is read three times, the second and third from cache
 template <typename T, bool RES> __global__ __launch_bounds__(1024) void fwd_wide_kernel(const LnP p) {
   __shared__ float red[16];
-  const long row = blockIdx.x;
+  const long row = p.row0 + blockIdx.x;
   const T* x = (const T*)p.x + row * p.ldx;
   float s[1] = {0.f};
   for (long c = threadIdx.x; c < p.W; c += 1024) {
@@ -326,13 +327,20 @@ __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ pa
     if (chunks <= 2048) return CALL(1024, 2);          \
   } while (0)
 
-template <typename T, int E, int LPR, int NC> int fwd_launch(const LnP& p, hipStream_t s) {
-  constexpr int kG = Block<LPR>::kThreads / LPR;
-  const dim3 grid((unsigned)((p.rows + kG - 1) / kG)), block(Block<LPR>::kThreads);
-  if (p.res) hipLaunchKernelGGL((fwd_kernel<T, E, LPR, NC, true>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((fwd_kernel<T, E, LPR, NC, false>), grid, block, 0, s, p);
-  OCEAN_LAUNCH_CHECK();
+// A grid holds fewer than 2^32 threads (more wrap around, with no error, and leave rows out): many short rows take several launches.
+constexpr long kMaxBlocks = 1L << 21;
+template <typename K> int launch_rows(K kernel, const LnP& p, int rows_a_block, int threads, hipStream_t s) {
+  LnP q = p;
+  for (q.row0 = 0; q.row0 < p.rows; q.row0 += kMaxBlocks * rows_a_block) {
+    const long blocks = (p.rows - q.row0 + rows_a_block - 1) / rows_a_block;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks)), dim3(threads), 0, s, q);
+    OCEAN_LAUNCH_CHECK();
+  }
   return OCEAN_OK;
+}
+template <typename T, int E, int LPR, int NC> int fwd_launch(const LnP& p, hipStream_t s) {
+  constexpr int kT = Block<LPR>::kThreads;
+  return launch_rows(p.res ? fwd_kernel<T, E, LPR, NC, true> : fwd_kernel<T, E, LPR, NC, false>, p, kT / LPR, kT, s);
 }
 template <typename T> int fwd_pick(const LnP& p, hipStream_t s) {
   constexpr int E = 16 / sizeof(T);
@@ -340,10 +348,7 @@ template <typename T> int fwd_pick(const LnP& p, hipStream_t s) {
 #define LN_CALL(LPR, NC) fwd_launch<T, E, LPR, NC>(p, s)
   LN_PICK_FWD(LN_CALL);
 #undef LN_CALL
-  if (p.res) hipLaunchKernelGGL((fwd_wide_kernel<T, true>), dim3((unsigned)p.rows), dim3(1024), 0, s, p);
-  else hipLaunchKernelGGL((fwd_wide_kernel<T, false>), dim3((unsigned)p.rows), dim3(1024), 0, s, p);
-  OCEAN_LAUNCH_CHECK();
-  return OCEAN_OK;
+  return launch_rows(p.res ? fwd_wide_kernel<T, true> : fwd_wide_kernel<T, false>, p, 1, 1024, s);
 }
 template <typename T, int E, int LPR, int NC> int bwd_launch(const LnP& p, hipStream_t s) {
   hipLaunchKernelGGL((bwd_kernel<T, E, LPR, NC>), dim3(p.blocks), dim3(Block<LPR>::kThreads), 0, s, p);
