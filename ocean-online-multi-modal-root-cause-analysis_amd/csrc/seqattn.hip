@@ -73,6 +73,9 @@ void plan_pieces(long units, long steps, bool causal, double slots, double tile_
   *per_piece = (int)((steps + *pieces - 1) / *pieces);
 }
 
+// A grid holds fewer than 2^32 threads (more wrap around, with no error): no launch may have more blocks of 256 than this.
+constexpr long kMaxBlocks = (1L << 24) - 1;
+
 struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
@@ -92,7 +95,7 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   }
   pl->D = (s->d + 31) / 32 * 32;
   const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
-  if (blocks > 0x7fffffffL / 16 || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL / 16) return OCEAN_ERR_UNSUPPORTED;
+  if (blocks > kMaxBlocks || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > kMaxBlocks) return OCEAN_ERR_UNSUPPORTED;
   // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as rows.
   pl->split = (long)s->Lq * G <= 32;
   pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
@@ -101,7 +104,6 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const long most = (s->Lk + 511) / 512;
   if (want > most) want = most;
   pl->splits = (int)(want < 1 ? 1 : want);
-  if (base * pl->splits > 0x7fffffffL) return OCEAN_ERR_UNSUPPORTED;
   pl->fwd_floats = pl->split && pl->splits > 1 ? (size_t)base * pl->splits * 32 * (pl->D + 2) : 0;
   if (!pl->split) {
     if (loose(s, s->k_strides, 1)) pl->fwd_floats += packed_floats(s, s->Hk, s->Lk);
@@ -125,6 +127,11 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const long tiles_of_keys = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;      // in pairs of equal work with `causal`
   plan_pieces((long)s->B * s->Hk * (s->causal ? (tiles_of_keys + 1) / 2 : tiles_of_keys), query_steps, false, slots,
               (b16 ? 2.9 * query_step / 32.0 : 17.0 * slots / 512.0) * wide, 128.0 * pl->D * 8, &pl->segs, &pl->seg_tiles);
+  const long units = (long)s->B * s->Hk * tiles_of_keys, pairs = (tiles_of_keys + 1) / 2;
+  const long most_blocks[] = {pl->split ? base * pl->splits : blocks * pl->parts, blocks * pl->dq_parts,
+                              (long)s->B * s->Hk * (s->causal ? 2 * pairs : tiles_of_keys) * pl->segs,
+                              (pl->parts > 1 || pl->dq_parts > 1) ? 4 * blocks : 0, pl->segs > 1 ? 4 * units : 0};
+  for (long n : most_blocks) if (n > kMaxBlocks) return OCEAN_ERR_UNSUPPORTED;
   if (!pl->split && pl->parts > 1) {
     pl->ml_at = pl->fwd_floats + (size_t)blocks * pl->parts * 128 * pl->D;
     pl->packed = pl->fwd_floats;

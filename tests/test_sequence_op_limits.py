@@ -1,0 +1,37 @@
+"""The largest and smallest that the sequence operators take, and what they answer beyond."""
+import ctypes
+
+import pytest
+import torch
+
+from ocean import _hip
+from test_sequence_op_refusals import attention_shape
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(B=1 << 24, H=1, Hk=1, Lq=1, Lk=1), 2), (dict(B=(1 << 24) - 1, H=1, Hk=1, Lq=1, Lk=1), 4), (dict(B=1 << 20, H=16, Hk=16, Lq=64, Lk=64), 2),
+    (dict(B=1 << 21, H=8, Hk=1, Lq=16, Lk=16), 2), (dict(B=1, H=1, Hk=1, Lq=40, Lk=1 << 30), 4), (dict(B=3, H=1, Hk=1, Lq=40, Lk=1 << 30), 2),
+    (dict(B=1, H=1, Hk=1, Lq=1 << 30, Lk=5), 4), (dict(B=1, H=2, Hk=2, Lq=1 << 30, Lk=5, causal=1), 2)])
+def test_more_blocks_than_a_grid_has_threads_for(change, status):
+    """2^24 blocks of 256 threads are 2^32, where a grid wraps around without an error."""
+    L, s = _hip.lib(), attention_shape(**change)
+    none = [None] * 7
+    assert L.ocean_attention_fwd(ctypes.byref(s), *none, None, 0, None, None, None) == status
+    assert L.ocean_attention_bwd(ctypes.byref(s), *none, None, None, None, None, 0, None, None, None, None, None) == status
+
+
+@pytest.mark.gpu
+def test_the_largest_batch():
+    from ocean import ops
+    B = (1 << 24) - 1
+    q, k, v, w = (torch.randn(8, device="cuda").bfloat16().expand(B, 1, 1, 8).contiguous() for _ in range(4))
+    v[-1], w[-1] = 7.0, 5.0
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = ops.attention(*leaves)                             # one key: its weight is 1
+    assert torch.equal(out, v)
+    dq, dk, dv = torch.autograd.grad(out, leaves, w)
+    # ds = p (dp - p dp) with p off from 1 by the rounding of the score t < 20 and of 2^x, (t + 2) 2^-24 at most; |dp| <= 280
+    assert torch.equal(dv, w) and max(dq.abs().max(), dk.abs().max()) <= 22 * 2.0 ** -24 * 280 / 8 ** 0.5 * max(q.abs().max(), k.abs().max())
+    with pytest.raises(_hip.OceanHipError, match="unsupported size"):
+        one = q.detach()[:1].expand(B + 1, 1, 1, 8)
+        ops.attention(one, one, one)
