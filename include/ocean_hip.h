@@ -586,7 +586,7 @@ typedef struct {
   int dtype;
   int causal;
   int query_start;
-  float scale;                     /* > 0 */
+  float scale;                     /* 1e-30 .. 1e30 */
   int num_buckets;                 /* 0: no position bias; at most 128 */
   int max_distance;                /* > E, at most 1024 */
   int bidirectional;

@@ -83,7 +83,8 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   if (!s) return OCEAN_ERR_NULL;
   if (s->B <= 0 || s->H <= 0 || s->Hk <= 0 || s->Lq <= 0 || s->Lk <= 0 || s->d <= 0 || s->H % s->Hk != 0) return OCEAN_ERR_BAD_SHAPE;
   if (s->dtype != OCEAN_F32 && s->dtype != OCEAN_BF16) return OCEAN_ERR_BAD_SHAPE;
-  if (!(s->scale > 0.f) || s->scale > 3.0e38f) return OCEAN_ERR_BAD_SHAPE;
+  // within these, scale * log2 e and the log-sums over it (where the launch over keys starts its products) stay finite
+  if (!(s->scale >= 1.0e-30f && s->scale <= 1.0e30f)) return OCEAN_ERR_BAD_SHAPE;
   if (s->d < (s->dtype == OCEAN_F32 ? 4 : 8) || s->d > 128) return OCEAN_ERR_UNSUPPORTED;
   if (s->Lq > (1 << 30) || s->Lk > (1 << 30) || s->query_start > (1 << 30) || s->query_start < -(1 << 30)) return OCEAN_ERR_UNSUPPORTED;
   const int G = s->H / s->Hk;

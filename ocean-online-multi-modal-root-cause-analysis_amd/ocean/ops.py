@@ -542,8 +542,8 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
     _gpu(key, "key", index)
     _gpu(value, "value", index)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale must be from 1e-30 to 1e30, got {scale}")
     if mask is not None:
         _gpu(mask, "mask", index)
         if mask.dtype not in (torch.bool, torch.uint8):

@@ -20,6 +20,33 @@ def test_more_blocks_than_a_grid_has_threads_for(change, status):
     assert L.ocean_attention_bwd(ctypes.byref(s), *none, None, None, None, None, 0, None, None, None, None, None) == status
 
 
+@pytest.mark.parametrize("scale,status", [(0.0, 1), (9e-31, 1), (1e-38, 1), (1.1e30, 1), (2.5e38, 1), (1e-30, 4), (1e30, 4)])
+def test_scales_whose_log2_form_or_inverse_is_not_finite(scale, status):
+    L, s = _hip.lib(), attention_shape(scale=scale)
+    none = [None] * 7
+    assert L.ocean_attention_fwd(ctypes.byref(s), *none, None, 0, None, None, None) == status
+    assert L.ocean_attention_bwd(ctypes.byref(s), *none, None, None, None, None, 0, None, None, None, None, None) == status
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_smallest_scale(dtype):
+    """Weights are all 1 / 200: the output is the values' mean and dv the gradient's."""
+    from ocean import ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    leaves = [torch.randn(1, 2, 200, 32, device="cuda", generator=g).to(dtype).requires_grad_(True) for _ in range(3)]
+    w = torch.randn(1, 2, 200, 32, device="cuda", generator=g).to(dtype)
+    for scale in (1e-38, 2.5e38):
+        with pytest.raises(ValueError):
+            ops.attention(*leaves, scale=scale)
+    out = ops.attention(*leaves, scale=1e-30)
+    u = torch.finfo(dtype).eps / 2                           # of the weights and of the result; 232 half steps of a sum of 200
+    for got, x in ((out, leaves[2]), (torch.autograd.grad(out, leaves, w)[2], w)):
+        x = x.detach().double()
+        size = x.abs().mean(2, keepdim=True)
+        assert ((got.double() - x.mean(2, keepdim=True)).abs() <= (232 * 2.0 ** -24 + 2 * u) * size).all()
+
+
 @pytest.mark.gpu
 def test_the_largest_batch():
     from ocean import ops
