@@ -50,7 +50,7 @@ struct Params {
   float* dtable_part;                // [H][B][key tiles][segments][buckets]
   int k_tiles, segs, seg_tiles;      // launch over keys: tiles of 128 keys, segments of their queries, query tiles (of all heads) a segment
   int splits; float* part_o; float* part_ml;     // partial results of split sums
-  int q_tiles;                       // tiles of 128 queries (over split keys: chunks of 32 rows)
+  int q_tiles;                       // tiles of 128 queries
   int parts, part_tiles;             // launches over queries: parts a query tile's keys are split into, key tiles a part
 };
 

@@ -76,7 +76,7 @@ void plan_pieces(long units, long steps, bool causal, double slots, double tile_
 // A grid holds fewer than 2^32 threads (more wrap around, with no error): no launch may have more blocks of 256 than this.
 constexpr long kMaxBlocks = (1L << 24) - 1;
 
-struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int chunks; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
+struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
   *pl = Plan{};
@@ -97,10 +97,9 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   pl->D = (s->d + 31) / 32 * 32;
   const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
   if (blocks > kMaxBlocks || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > kMaxBlocks) return OCEAN_ERR_UNSUPPORTED;
-  // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as rows.
+  // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as one block's rows.
   pl->split = (long)s->Lq * G <= 32;
-  pl->chunks = (int)(((long)s->Lq * G + 31) / 32);
-  const long base = (long)s->B * s->Hk * pl->chunks;
+  const long base = (long)s->B * s->Hk;
   long want = (512 + base - 1) / base;
   const long most = (s->Lk + 511) / 512;
   if (want > most) want = most;
@@ -189,8 +188,7 @@ int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const voi
   p.lse = lse;
   if (pl.split) {
     p.splits = pl.splits;
-    p.q_tiles = pl.chunks;
-    const size_t rows = (size_t)s->B * s->Hk * pl.chunks * pl.splits * 32;
+    const size_t rows = (size_t)s->B * s->Hk * pl.splits * 32;
     p.part_o = ws;
     p.part_ml = ws + rows * pl.D;
   } else {

@@ -175,8 +175,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 }
 
 // ---------------------------------------------------------------- few queries: the keys are split
-// A block's 32 rows are (query, head of the group) pairs of one key head, so a single token's G heads read the keys once; its
-// four waves take 32-key tiles in turn, each through LDS of its own, and the blocks of one row chunk split the keys further.
+// A block's 32 rows are the (query, head of the group) pairs of one key head (at most so many: launch plan), so a single token's G
+// heads read the keys once; its four waves take 32-key tiles in turn, each through LDS of its own, and the blocks of a key head split
+// the keys further.
 // Bound by reading the keys and values once: 16 samples x 8 key heads x up to 16384 keys x 128 bf16, 698 MB, 138 us = 5.1 TB/s, what
 // a large copy reaches; a short cache (257 keys) by latency, 7.8 us.
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void fwd_split_kernel(const Params p) {
@@ -186,10 +187,9 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   char* const kt = smem + w * 2 * 32 * TL::kRowBytes;
   char* const vt = kt + 32 * TL::kRowBytes;
   uint8_t* const bmap = reinterpret_cast<uint8_t*>(smem + 8 * 32 * TL::kRowBytes);
-  const int split = blockIdx.x % p.splits, chunk_id = blockIdx.x / p.splits;
-  const int chunks = p.q_tiles, chunk = chunk_id % chunks, bk = chunk_id / chunks, b = bk / p.Hk, kh = bk % p.Hk;
+  const int split = blockIdx.x % p.splits, bk = blockIdx.x / p.splits, b = bk / p.Hk, kh = bk % p.Hk;
   const int keys = keys_of(p, b), start = start_of(p, b);
-  const int m = chunk * 32 + (lane & 31), i = m / p.G, head = kh * p.G + m % p.G, pos = start + i;
+  const int m = lane & 31, i = m / p.G, head = kh * p.G + m % p.G, pos = start + i;
   const bool live = m < p.Lq * p.G;
   if (BIAS) {
     for (int x = tid; x <= 2 * p.max_dist; x += 256) bmap[x] = (uint8_t)bucket_of(p, x - p.max_dist);
@@ -206,9 +206,8 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   RowRegs<T, D> q;
   q.load(own ? (const T*)p.q.p + b * p.q.b + head * p.q.h + (long)i * p.q.l : nullptr, p.d, lane);
   const uint8_t* mrow = MASK && live ? p.mask + b * p.mb + head * p.mh + (long)i * p.mi : nullptr;
-  const int last = start + min((chunk * 32 + 31) / p.G, p.Lq - 1);
-  const int end = p.causal ? min(keys, last + 1) : keys;
-  const int full = p.causal ? min(keys, start + chunk * 32 / p.G + 1) : keys;
+  const int end = p.causal ? min(keys, start + p.Lq) : keys;
+  const int full = p.causal ? min(keys, start + 1) : keys;
   const int tiles = end > 0 ? (end + 31) / 32 : 0, per = (tiles + p.splits - 1) / p.splits;
   const int t1 = min(tiles, (split + 1) * per);
   const float c = p.scale * kLog2e, mult = BIAS ? 1.f : c;
@@ -229,17 +228,20 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
       ks.fetch(kb, p.k.l, 32 * (t + 4), keys, p.d, lane, kk);
       vs.fetch(vb, p.v.l, 32 * (t + 4), keys, p.d, lane, kk);
     }
+    const int j0 = 32 * t;
+    f32x16 bias;                                            // read in front of the fence: sixteen loads in flight, not one by one
+    if (BIAS) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        bias[r] = p.table[(long)bmap[dist_slot(p, j0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) - pos)] * p.H + min(head, p.H - 1)];
+    }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int j0 = 32 * t;
     f32x16 s[1];
     s[0] = row_mma<T, D>(kt, 0, lane, q, f32x16{});
     if (BIAS) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int dist = j0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) - pos;
-        s[0][r] = fmaf(s[0][r], c, p.table[(long)bmap[dist_slot(p, dist)] * p.H + min(head, p.H - 1)] * kLog2e);
-      }
+      for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], c, bias[r] * kLog2e);
     }
     adjust<false, MASK>(p, s[0], c, j0, pos, 0, keys, mrow, nullptr, j0 + 32 > full, lane);
     const float f = softmax_step<1>(s, mult, st);
@@ -266,7 +268,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     for (int r = 0; r < 16; ++r) ob[(w * D + db * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * 32 + (lane & 31)] = acc[db][r];
   __syncthreads();
   const int row = tid & 31;
-  const int mr = chunk * 32 + row, ir = mr / p.G, hr = kh * p.G + mr % p.G;
+  const int ir = row / p.G, hr = kh * p.G + row % p.G;
   float mx = -INFINITY;
 #pragma unroll
   for (int v = 0; v < 4; ++v) mx = fmaxf(mx, ml[v * 64 + row]);
@@ -276,10 +278,10 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
     fw[v] = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[v * 64 + row] - mx);
     lt += fw[v] * ml[v * 64 + 32 + row];
   }
-  if (mr >= p.Lq * p.G) return;
+  if (row >= p.Lq * p.G) return;
   const bool whole = p.splits == 1;
   const float inv = !whole ? 1.f : lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-  const long pr = ((long)chunk_id * p.splits + split) * 32 + row;
+  const long pr = ((long)bk * p.splits + split) * 32 + row;
   T* out = (T*)p.o.p + b * p.o.b + hr * p.o.h + (long)ir * p.o.l;
   for (int e0 = 4 * (tid >> 5); e0 < D; e0 += 32) {
     float x[4];
@@ -305,7 +307,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void fwd_join_ker
   if (n >= rows) return;
   const int rg = p.Lq * p.G, m = (int)(n % rg), bk = (int)(n / rg), b = bk / p.Hk, kh = bk % p.Hk;
   const int i = m / p.G, head = kh * p.G + m % p.G;
-  const long first = ((long)(bk * p.q_tiles + m / 32) * p.splits) * 32 + (m & 31);
+  const long first = (long)bk * p.splits * 32 + m;
   float mx = -INFINITY;
   for (int s = lane; s < p.splits; s += 64) mx = fmaxf(mx, p.part_ml[2 * (first + (long)s * 32)]);
 #pragma unroll
@@ -351,7 +353,7 @@ template <typename T, int D, bool BIAS, bool MASK> int forward(const Params& p, 
   const size_t meet = (size_t)(4 * D * 32 + 4 * 2 * 32) * sizeof(float);
   if (meet > lds) lds = meet;
   OCEAN_TRY(set_lds(fwd_split_kernel<T, D, BIAS, MASK>, lds));
-  hipLaunchKernelGGL((fwd_split_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.Hk * p.q_tiles * p.splits)), dim3(256), lds, s, p);
+  hipLaunchKernelGGL((fwd_split_kernel<T, D, BIAS, MASK>), dim3((unsigned)((long)p.B * p.Hk * p.splits)), dim3(256), lds, s, p);
   OCEAN_LAUNCH_CHECK();
   if (p.splits > 1) {
     hipLaunchKernelGGL((fwd_join_kernel<T, D>), dim3((unsigned)(((long)p.B * p.H * p.Lq + 3) / 4)), dim3(256), 0, s, p);
