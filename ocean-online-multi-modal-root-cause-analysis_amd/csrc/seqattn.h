@@ -87,25 +87,31 @@ template <typename T, int D> struct Tile {
   }
 };
 
-// the 16 probabilities of a lane as the right operand of a product over the 32 rows they stand for
-template <typename T> struct PFrag;
-template <> struct PFrag<__bf16> {
-  bf16x8 f[2];
-  // rounded to bf16 (half a step, 2^-9 of each weight): the matrix instruction takes both operands in one type; sums stay fp32
+// The 16 probabilities of a lane as the right operand of a product over the 32 rows they stand for.  The matrix instruction takes
+// both operands in one type, so 16-bit inputs' probabilities are rounded to bf16: half a step, up to 2^-8 of each weight, where sums and
+// statistics stay fp32.  FINE adds the product of what the rounding left, and 2^-16 remain: where the kernel waits for memory
+// that is free (16 tokens over 16384 keys x 128: 139 -> 140 us), where it waits for matrix cores it is not (prompt of 8192: 298 -> 420 us,
+// training step 2 x 4096: 756 -> 1028 us), and a bf16 output is 1.4 times as far from exact as its own rounding alone.
+template <typename T, bool FINE = false> struct PFrag;
+template <bool FINE> struct PFrag<__bf16, FINE> {
+  bf16x8 f[2], rest[2];
   __device__ __forceinline__ void set(const f32x16& p) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[s][e] = (__bf16)p[8 * s + e];
+      for (int e = 0; e < 8; ++e) {
+        f[s][e] = (__bf16)p[8 * s + e];
+        if (FINE) rest[s][e] = (__bf16)(p[8 * s + e] - (float)f[s][e]);
+      }
   }
 };
-template <> struct PFrag<float> {
+template <bool FINE> struct PFrag<float, FINE> {
   f32x16 f;
   __device__ __forceinline__ void set(const f32x16& p) { f = p; }
 };
 
 // acc[c][col] += sum over the 32 rows row0.. of tile[row][32 db + c] * p[row][col]
-template <int D> __device__ __forceinline__ f32x16 col_mma(const char* t, int row0, int db, int lane, const PFrag<__bf16>& p, f32x16 acc) {
+template <int D, bool FINE> __device__ __forceinline__ f32x16 col_mma(const char* t, int row0, int db, int lane, const PFrag<__bf16, FINE>& p, f32x16 acc) {
   typedef Tile<__bf16, D> TL;
   const int gl = lane & 15, grp = lane >> 4;
   const int chunk = db * 4 + 2 * (grp & 1) + ((gl & 3) >> 1), sub = (gl & 1) * 8;
@@ -118,10 +124,11 @@ template <int D> __device__ __forceinline__ f32x16 col_mma(const char* t, int ro
     const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), h4 = __builtin_bit_cast(bf16x4, hi);
     const bf16x8 a = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
     acc = Mm<__bf16>::mma(a, p.f[s], acc);
+    if (FINE) acc = Mm<__bf16>::mma(a, p.rest[s], acc);
   }
   return acc;
 }
-template <int D> __device__ __forceinline__ f32x16 col_mma(const char* t, int row0, int db, int lane, const PFrag<float>& p, f32x16 acc) {
+template <int D, bool FINE> __device__ __forceinline__ f32x16 col_mma(const char* t, int row0, int db, int lane, const PFrag<float, FINE>& p, f32x16 acc) {
   typedef Tile<float, D> TL;
   const int c = db * 32 + (lane & 31), h = lane >> 5;
 #pragma unroll
@@ -187,7 +194,7 @@ template <typename T, int D, int ROWS, int THREADS> struct Stage {
 
 // The same tile straight from global memory into LDS, 16 bytes a lane, in flight until wait_tiles(): no registers, no LDS
 // writes.  A wave's 64 lanes fill 1024 consecutive bytes, so the permutation within a row is made on the global side.  Needs
-// 16-byte aligned rows of whole chunks (Params::whole); rows and features past the end come from a line of zeros.
+// 16-byte aligned rows of whole chunks (the entry points copy other inputs into the workspace first); rows and features past the end come from a line of zeros.
 static __device__ const u32x4 kZeros[1] = {{0u, 0u, 0u, 0u}};
 template <typename T, int D, int ROWS, int THREADS> struct Async {
   typedef Tile<T, D> TL;

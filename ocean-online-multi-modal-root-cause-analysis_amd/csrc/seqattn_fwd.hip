@@ -249,7 +249,7 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) acc[db] *= f;
     }
-    PFrag<T> pf;
+    PFrag<T, true> pf;
     pf.set(s[0]);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) acc[db] = col_mma<D>(vt, 0, db, lane, pf, acc[db]);

@@ -60,3 +60,17 @@ def test_layer_norm_keeps_the_deviation_of_rows_far_from_zero(W):
     assert (shift.abs() <= e * rstd + u).all()
     rel = (e * e / var + 48 * u) / 2 + 4 * u                 # of the deviation's inverse; its root, quotient and product
     assert ((y - shift - xc * rstd).abs() <= rel * (xc * rstd).abs() + (rel + u) * e * rstd + u * y.abs() + 2 * u).all()
+
+
+@pytest.mark.parametrize("B,H,Hk,Lq,Lk,d", [(1, 8, 2, 1, 257, 64), (3, 8, 1, 1, 5000, 128), (2, 4, 2, 9, 777, 40)])
+def test_single_tokens_in_bf16_round_once(B, H, Hk, Lq, Lk, d):
+    """The weights of few queries keep 16 bits (2^-16 of each), so only the output's own rounding is a bf16 one."""
+    from ocean import ops
+    g = torch.Generator(device="cuda").manual_seed(Lk)
+    q, k, v = (torch.randn(B, h, n, d, device="cuda", generator=g).bfloat16() for h, n in ((H, Lq), (Hk, Lk), (Hk, Lk)))
+    ok, _ = ref.places(B, H, Lq, Lk)
+    r = ref.attention(q, k, v, ok, 1 / math.sqrt(d))
+    limit = ref.tolerance("out", r, torch.float32, d, Lk) + 2.0 ** -16 * r["mag"]["out"]
+    limit = limit + 2.0 ** -8 * (r["out"].abs() + limit)
+    err = (ops.attention(q, k, v).double() - r["out"]).abs()
+    assert (err <= limit).all(), f"{(err / limit).amax().item():.3g} times the bound"
