@@ -252,7 +252,9 @@ template <typename T, int E, int LPR, int NC> __global__ __launch_bounds__(Block
   }
 }
 
-// wide rows: the columns' sums live in the block's line of the workspace, which only this block writes
+// wide rows: the columns' sums live in the block's line of the workspace, which only this block writes.  Single values a load, and a
+// read and a write of both sums for every row: 2048 rows of 16384 fp32 take 321 us, 1024 of 32768 336 us, 2048 of 32768 bf16 568 us,
+// where x and dy read twice and dx written would be 131 us at a large copy's rate.
 template <typename T> __global__ __launch_bounds__(1024) void bwd_wide_kernel(const LnP p) {
   __shared__ float red[32];
   float* pw = p.part ? p.part + (long)blockIdx.x * 2 * p.W : nullptr;

@@ -117,7 +117,8 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const size_t rows = (size_t)s->B * s->H * s->Lq;
   pl->delta_at = at;
   pl->parts_at = at + ((rows + 3) & ~size_t(3));
-  // rates measured with the chip full: a step is 64 (32 in fp32) keys or queries of a tile of 128
+  // Rates measured with the chip full, at 96 and 128 features: a step is 64 (32 in fp32) keys or queries of a tile of 128.  Samples
+  // count as Lk keys long, and the forward launch as two blocks a compute unit, also where its build (fp32 or a mask at 128) holds one.
   const bool b16 = s->dtype != OCEAN_F32;
   const int key_step = seqattn::key_tile(b16), row_bytes = pl->D * (b16 ? 2 : 4), query_step = seqattn::query_tile(row_bytes);
   const double wide = pl->D / 128.0, slots = row_bytes > 256 ? 256.0 : 512.0;

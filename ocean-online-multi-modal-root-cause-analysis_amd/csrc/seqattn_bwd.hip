@@ -121,9 +121,9 @@ template <typename T, int D> struct BwdTile {
 };
 
 // Launch over queries, three products (s, dp, dq): the wave's 32 queries and their d_out in registers, keys and values through two
-// LDS buffers each.  Bound by the turns of its two waves a SIMD between matrix cores (busy 0.44 of the cycles), vector units (0.36)
-// and tiles (waiting 0.40); the registers hold no third wave and no second tile.  Causal 2 x 16
-// heads (4 of keys) x 4096 x 128 bf16: 235 us = 0.88 PFLOP/s of the three products; 8 x 8 heads x 512 x 96 fp32, ragged: 97 us.
+// LDS buffers each.  Bound by the turns of its two waves a SIMD between matrix cores (busy 0.45 of the cycles), vector units (0.37), LDS
+// (0.45, half of it bank conflicts) and tiles (waiting 0.40); the registers hold no third wave and no second tile.  Causal 2 x 16
+// heads (4 of keys) x 4096 x 128 bf16: 228 us = 0.90 PFLOP/s of the three products; 8 x 8 heads x 512 x 96 fp32, ragged: 96 us.
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void dq_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BN = BwdTile<T, D>::kKeys, NS = BN / 32;
@@ -288,8 +288,12 @@ template <int BM> __device__ __forceinline__ Span span_of(const Params& p, int t
 
 // A wave keeps its 32 keys' dk and dv in registers, and the keys as right operand; the values too where that leaves room for two
 // waves on a SIMD, else they stay in LDS (VL): at 128 16-bit features the registers of both were 440, and half of the instructions
-// moved accumulators between the two register files.  Four products (s, dp, dv, dk).  Bound as the launch over queries is: causal
-// 2 x 16 heads (4 of keys) x 4096 x 128 bf16: 425 us = 0.65 PFLOP/s of the four; 8 x 8 heads x 512 x 96 fp32, ragged: 135 us.
+// moved accumulators between the two register files.  Four products (s, dp, dv, dk).  The 256 registers of two waves a SIMD still do
+// not hold it at 96 and 128 16-bit features: 16 bytes a lane live in scratch memory at 128 (8 with a mask, 20 with a bias, 84 with both),
+// 40 at 96 (28, 80, 152).  Causal 2 x 16 heads (4 of keys) x 4096 x 128 bf16: 419 us = 0.66 PFLOP/s of the four, bound by waiting for LDS
+// and barriers with few waves (1.44 a SIMD, waiting 0.52 of their cycles; LDS busy 0.43 of the cycles, 0.19 in bank conflicts; matrix
+// cores 0.31, vector 0.20).  16 x 12 heads x 512 x 64 with a bias, ragged: 77 us, waiting too (0.51, 1.2 waves a SIMD; matrix cores 0.11,
+// vector 0.25).  8 x 8 heads x 512 x 96 fp32, ragged: 134 us, 0.7 waves a SIMD between their own matrix instructions (busy 0.45).
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void dkv_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BM = BwdTile<T, D>::kRows, NS = BM / 32;

@@ -85,9 +85,11 @@ template <typename T, int D> __global__ __launch_bounds__(256) void fwd_rows_joi
 }
 
 // One block a query tile: the wave's 32 queries stay in registers as the right operand, keys and values pass through two LDS buffers,
-// the next tile loading while this one is used.  Bound in bf16 by the turns of two waves a SIMD between matrix cores (busy 0.39 of
-// the cycles) and the softmax's vector instructions (0.42), in fp32 by the matrix cores' own rate.  Causal 16 heads (4 of keys) x 8192 x 128 bf16: 285 to 320 us (with the clock), 0.96 to 0.86
-// PFLOP/s of the pairs' 4 d, of 1.21 that a large product reaches; 2 x 16 heads x 4096: 170 us; 8 x 8 heads x 512 x 96 fp32, ragged: 68 us.
+// the next tile loading while this one is used.  Bound in bf16 by the turns of two waves a SIMD between matrix cores (busy 0.40 of
+// the cycles), the softmax's vector instructions (0.42) and LDS (0.40, half of it bank conflicts).  Causal 16 heads (4 of keys) x 8192 x
+// 128 bf16: 285 to 330 us (with the clock), 0.96 to 0.83 PFLOP/s of the pairs' 4 d, of 1.21 that a large product reaches; 2 x 16 heads x
+// 4096: 171 us.  8 x 8 heads x 512 x 96 fp32, ragged: 67 us; short samples leave 1.07 waves a SIMD, which spend 0.69 of their cycles
+// waiting for their turn, most of it for their own last matrix instruction (matrix cores busy 0.43).
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > (MASK ? 128 : 256) ? 1 : 2) void fwd_rows_kernel(const Params p) {
   typedef Tile<T, D> TL;
   constexpr int BN = FwdTile<T, D>::kKeys, NS = BN / 32;
@@ -179,7 +181,8 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
 // heads read the keys once; its four waves take 32-key tiles in turn, each through LDS of its own, and the blocks of a key head split
 // the keys further.
 // Bound by reading the keys and values once: 16 samples x 8 key heads x up to 16384 keys x 128 bf16, 698 MB, 138 us = 5.1 TB/s, what
-// a large copy reaches; a short cache (257 keys) by latency, 7.8 us.
+// a large copy reaches; a short cache (257 keys) by latency, 8.0 us.  fp32, all 16384 keys: 265 us at 64 features (4.1 TB/s), 492 us at
+// 128 (4.4 TB/s), where its registers (256 and 145 or more from 96 features on) leave one wave a SIMD to load ahead.
 template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(256, D * sizeof(T) > 256 ? 1 : 2) void fwd_split_kernel(const Params p) {
   typedef Tile<T, D> TL;
   extern __shared__ __attribute__((aligned(16))) char smem[];
