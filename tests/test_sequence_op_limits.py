@@ -48,6 +48,21 @@ def test_the_smallest_scale(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Lq", [1, 150])
+def test_scaled_scores_of_nine_hundred_millions(dtype, Lq):
+    """One key at 9.1e8, the others at half: its weight is 1, and the remaining exponent, a rounding of 1.3e9, is 64 at most."""
+    from ocean import ops
+    q = torch.full((1, 2, Lq, 32), 2.0 ** 14, device="cuda", dtype=dtype)
+    k = torch.full((1, 1, 300, 32), 2.0 ** 9, device="cuda", dtype=dtype)
+    k[:, :, 170] *= 2
+    v = torch.randn(1, 1, 300, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    out = ops.attention(q, k, v, scale=1.7).double()
+    want = v[:, :, 170:171].double()                         # (e v) / e: three roundings and their products, in bf16 of e and out too
+    assert ((out - want).abs() <= (4 * 2.0 ** -24 + (0 if dtype == torch.float32 else 2.01 * 2.0 ** -8)) * want.abs()).all()
+
+
+@pytest.mark.gpu
 def test_the_largest_batch():
     from ocean import ops
     B = (1 << 24) - 1
