@@ -568,7 +568,8 @@ int ocean_clip_adam_step_auto(const ocean_adam_chunk* table, int n_chunks, ocean
  * `starts`) among the keys.  Allowed: j < lengths[b] (clamped to 0..Lk; NULL: Lk), with causal j <= the query's position, and
  * with a mask mask[b, h, i, j] != 0.  Keys and values past a sample's length are not read, nor are those that a mask of query
  * stride 0 (and head stride 0 when key heads are shared) takes, nor queries that one of key stride 0 takes.  Query head h reads key head
- * h / (H / Hk).  Positions are int32, |position| < 2^30.  B * H * ceil(Lq / 128) and B * Hk * ceil(Lk / 128) are below 2^24.
+ * h / (H / Hk).  Positions are int32, |position| < 2^30.  B * H * ceil(Lq / 128) and B * Hk * ceil(Lk / 128) are below 2^24
+ * (in a forward call without lse only the first, or B * Hk where Lq * H / Hk <= 32).
  * Position bias: table[bucket(j - position)][h] is added to the score.  With side = num_buckets (bidirectional: half of them for
  * each sign, the upper half for keys after the query) and E = side / 2, distances n < E have a bucket each, farther ones share
  * E + floor((side - E) ln(n / E) / ln(max_distance / E)), at most side - 1; one-sided, keys after the query count as n = 0.

@@ -76,7 +76,7 @@ void plan_pieces(long units, long steps, bool causal, double slots, double tile_
 // A grid holds fewer than 2^32 threads (more wrap around, with no error): no launch may have more blocks of 256 than this.
 constexpr long kMaxBlocks = (1L << 24) - 1;
 
-struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int splits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
+struct Plan { int parts, part_tiles, dq_parts, dq_part_tiles, segs, seg_tiles; size_t part_at, ml_at, packed; int D; int split; int splits; bool fwd_fits, bwd_fits; size_t fwd_floats, bwd_floats, delta_at, parts_at; };
 
 int plan_of(const ocean_attention_shape* s, Plan* pl) {
   *pl = Plan{};
@@ -96,7 +96,7 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   }
   pl->D = (s->d + 31) / 32 * 32;
   const long q_tiles = (s->Lq + 127) / 128, blocks = (long)s->B * s->H * q_tiles;
-  if (blocks > kMaxBlocks || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > kMaxBlocks) return OCEAN_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffffL / 16 || (long)s->B * s->Hk * ((s->Lk + 127) / 128) > 0x7fffffffL / 16) return OCEAN_ERR_UNSUPPORTED;
   // Few queries take the kernel that splits the keys over blocks and packs the heads of a group as one block's rows.
   pl->split = (long)s->Lq * G <= 32;
   const long base = (long)s->B * s->Hk;
@@ -128,11 +128,11 @@ int plan_of(const ocean_attention_shape* s, Plan* pl) {
   const long tiles_of_keys = (s->Lk + seqattn::kKeyTile - 1) / seqattn::kKeyTile;      // in pairs of equal work with `causal`
   plan_pieces((long)s->B * s->Hk * (s->causal ? (tiles_of_keys + 1) / 2 : tiles_of_keys), query_steps, false, slots,
               (b16 ? 2.9 * query_step / 32.0 : 17.0 * slots / 512.0) * wide, 128.0 * pl->D * 8, &pl->segs, &pl->seg_tiles);
-  const long units = (long)s->B * s->Hk * tiles_of_keys, pairs = (tiles_of_keys + 1) / 2;
-  const long most_blocks[] = {pl->split ? base * pl->splits : blocks * pl->parts, blocks * pl->dq_parts,
-                              (long)s->B * s->Hk * (s->causal ? 2 * pairs : tiles_of_keys) * pl->segs,
-                              (pl->parts > 1 || pl->dq_parts > 1) ? 4 * blocks : 0, pl->segs > 1 ? 4 * units : 0};
-  for (long n : most_blocks) if (n > kMaxBlocks) return OCEAN_ERR_UNSUPPORTED;
+  // the launches and, where there are several pieces, those that join them
+  const long with_join = pl->parts > 4 ? pl->parts : pl->parts > 1 ? 4 : 1, dq_with_join = pl->dq_parts > 4 ? pl->dq_parts : pl->dq_parts > 1 ? 4 : 1;
+  const long key_tiles = base * (s->causal ? (tiles_of_keys + 1) / 2 * 2 : tiles_of_keys), dkv_with_join = pl->segs > 4 ? pl->segs : pl->segs > 1 ? 4 : 1;
+  pl->fwd_fits = (pl->split ? base * pl->splits : blocks * with_join) <= kMaxBlocks;
+  pl->bwd_fits = blocks * dq_with_join <= kMaxBlocks && key_tiles * dkv_with_join <= kMaxBlocks;
   if (!pl->split && pl->parts > 1) {
     pl->ml_at = pl->fwd_floats + (size_t)blocks * pl->parts * 128 * pl->D;
     pl->packed = pl->fwd_floats;
@@ -181,6 +181,7 @@ int ocean_attention_fwd(const ocean_attention_shape* s, const void* q, const voi
   Plan pl;
   Params p;
   OCEAN_TRY(plan_of(s, &pl));
+  if (!pl.fwd_fits || (lse && !pl.bwd_fits)) return OCEAN_ERR_UNSUPPORTED;
   OCEAN_TRY(fill(s, pl, q, k, v, mask, lengths, starts, table, &p));
   if (!out || (pl.fwd_floats && !ws)) return OCEAN_ERR_NULL;
   if (ws_floats < pl.fwd_floats) return OCEAN_ERR_WORKSPACE;
@@ -209,6 +210,7 @@ int ocean_attention_bwd(const ocean_attention_shape* s, const void* q, const voi
   Plan pl;
   Params p;
   OCEAN_TRY(plan_of(s, &pl));
+  if (!pl.bwd_fits) return OCEAN_ERR_UNSUPPORTED;
   OCEAN_TRY(fill(s, pl, q, k, v, mask, lengths, starts, table, &p));
   if (!out || !lse || !d_out || !ws || (dtable && !table)) return OCEAN_ERR_NULL;
   if (ws_floats < pl.bwd_floats) return OCEAN_ERR_WORKSPACE;

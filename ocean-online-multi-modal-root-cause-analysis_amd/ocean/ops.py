@@ -512,7 +512,7 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ma
     query [batch, heads, queries, d], key / value [batch, key heads, keys, d] in fp32 or bf16, d at most 128, any strides (a
     transposed view of a projection's [batch, length, heads * d] needs no copy; the result has the query's memory order).
     Query heads share key heads in equal groups; batch * heads * ceil(queries / 128), and the same of key heads and keys, are below
-    2^24.  Products and sums accumulate in fp32; the probabilities enter the second
+    2^24 (without gradients only the first, or batch * key heads for up to 32 queries a key head).  Products and sums accumulate in fp32; the probabilities enter the second
     product in the inputs' type.
 
     mask: bool or uint8, broadcastable to [batch, heads, queries, keys], nonzero = allowed.  key_lengths: int32 [batch] on the

@@ -8,16 +8,18 @@ from ocean import _hip
 from test_sequence_op_refusals import attention_shape
 
 
-@pytest.mark.parametrize("change,status", [
-    (dict(B=1 << 24, H=1, Hk=1, Lq=1, Lk=1), 2), (dict(B=(1 << 24) - 1, H=1, Hk=1, Lq=1, Lk=1), 4), (dict(B=1 << 20, H=16, Hk=16, Lq=64, Lk=64), 2),
-    (dict(B=1 << 21, H=8, Hk=1, Lq=16, Lk=16), 2), (dict(B=1, H=1, Hk=1, Lq=40, Lk=1 << 30), 4), (dict(B=3, H=1, Hk=1, Lq=40, Lk=1 << 30), 2),
-    (dict(B=1, H=1, Hk=1, Lq=1 << 30, Lk=5), 4), (dict(B=1, H=2, Hk=2, Lq=1 << 30, Lk=5, causal=1), 2)])
-def test_more_blocks_than_a_grid_has_threads_for(change, status):
-    """2^24 blocks of 256 threads are 2^32, where a grid wraps around without an error."""
+@pytest.mark.parametrize("change,forward,backward", [
+    (dict(B=1 << 24, H=1, Hk=1, Lq=1, Lk=1), 2, 2), (dict(B=(1 << 24) - 1, H=1, Hk=1, Lq=1, Lk=1), 4, 4), (dict(B=1 << 20, H=16, Hk=16, Lq=64, Lk=64), 2, 2),
+    (dict(B=1 << 21, H=8, Hk=1, Lq=16, Lk=16), 2, 2), (dict(B=1 << 21, H=8, Hk=1, Lq=4, Lk=16), 4, 2), (dict(B=1, H=1, Hk=1, Lq=40, Lk=1 << 30), 4, 4),
+    (dict(B=3, H=1, Hk=1, Lq=40, Lk=1 << 30), 4, 2), (dict(B=1, H=1, Hk=1, Lq=1 << 30, Lk=5), 4, 4), (dict(B=1, H=2, Hk=2, Lq=1 << 30, Lk=5, causal=1), 2, 2)])
+def test_more_blocks_than_a_grid_has_threads_for(change, forward, backward):
+    """2^24 blocks of 256 threads are 2^32, where a grid wraps around without an error.  A forward call that leaves lse is one that
+    a backward call follows."""
     L, s = _hip.lib(), attention_shape(**change)
-    none = [None] * 7
-    assert L.ocean_attention_fwd(ctypes.byref(s), *none, None, 0, None, None, None) == status
-    assert L.ocean_attention_bwd(ctypes.byref(s), *none, None, None, None, None, 0, None, None, None, None, None) == status
+    none, lse = [None] * 7, ctypes.c_void_p(64)
+    assert L.ocean_attention_fwd(ctypes.byref(s), *none, None, 0, None, None, None) == forward
+    assert L.ocean_attention_fwd(ctypes.byref(s), *none, None, 0, None, lse, None) == max((forward, backward), key=lambda x: x == 2)
+    assert L.ocean_attention_bwd(ctypes.byref(s), *none, None, None, None, None, 0, None, None, None, None, None) == backward
 
 
 @pytest.mark.parametrize("scale,status", [(0.0, 1), (9e-31, 1), (1e-38, 1), (1.1e30, 1), (2.5e38, 1), (1e-30, 4), (1e30, 4)])
@@ -77,3 +79,15 @@ def test_the_largest_batch():
     with pytest.raises(_hip.OceanHipError, match="unsupported size"):
         one = q.detach()[:1].expand(B + 1, 1, 1, 8)
         ops.attention(one, one, one)
+
+
+@pytest.mark.gpu
+def test_a_large_batch_of_single_tokens_with_shared_key_heads():
+    """2^24 query heads on 2^21 key heads: the forward call alone takes them, one that gradients follow does not."""
+    from ocean import ops
+    B = 1 << 21
+    q = torch.randn(B, 8, 1, 8, device="cuda").bfloat16()
+    k, v = (torch.randn(B, 1, 1, 8, device="cuda").bfloat16() for _ in range(2))
+    assert torch.equal(ops.attention(q, k, v), v.expand(B, 8, 1, 8))
+    with pytest.raises(_hip.OceanHipError, match="unsupported size"):
+        ops.attention(q.requires_grad_(True), k, v)
