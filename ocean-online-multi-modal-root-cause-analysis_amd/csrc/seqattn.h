@@ -405,6 +405,13 @@ template <int D> __device__ __forceinline__ void store_part(float* part, const f
 // and where piece n of lane's row goes: features part_feature(..).. + 3
 __device__ __forceinline__ int part_feature(int n, int lane) { return n / 4 * 32 + 8 * (n & 3) + 4 * (lane >> 5); }
 
+// a launch with more than the default 64 KB of LDS has to say so
+template <typename K> int set_lds(K kernel, size_t bytes) {
+  if (bytes <= 65536) return OCEAN_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
+}
+
 int launch_forward(const Params& p, int type, hipStream_t s);
 int launch_backward(const Params& p, int type, float* dtable, hipStream_t s);
 

@@ -527,12 +527,6 @@ __global__ __launch_bounds__(256) void dtable_kernel(const float* __restrict__ p
   if (threadIdx.x == 0) out[(long)k * H + head] = (float)red[0];
 }
 
-template <typename K> int set_lds(K kernel, size_t bytes) {
-  if (bytes <= 65536) return OCEAN_OK;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
-}
-
 template <typename T, int D, bool BIAS, bool MASK> int backward(const Params& p, float* dtable, hipStream_t s) {
   typedef Tile<T, D> TL;
   constexpr int BN = BwdTile<T, D>::kKeys, BM = BwdTile<T, D>::kRows;

@@ -333,12 +333,6 @@ template <typename T, int D> __global__ __launch_bounds__(256) void fwd_join_ker
   if (p.lse && lane == 0) p.lse[((long)b * p.H + head) * p.Lq + i] = l == 0.f ? INFINITY : mx + __builtin_amdgcn_logf(l);
 }
 
-template <typename K> int set_lds(K kernel, size_t bytes) {
-  if (bytes <= 65536) return OCEAN_OK;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == hipSuccess ? OCEAN_OK : OCEAN_ERR_HIP + (int)e;
-}
-
 template <typename T, int D, bool BIAS, bool MASK> int forward(const Params& p, hipStream_t s) {
   typedef Tile<T, D> TL;
   if (p.splits == 0) {
