@@ -220,17 +220,28 @@ template <typename T, int D, bool BIAS, bool MASK> __global__ __launch_bounds__(
   for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
   Stage<T, D, 32, 64> ks, vs;
   int t = split * per + w;
-  if (t < t1) {
-    ks.fetch(kb, p.k.l, 32 * t, keys, p.d, lane, kk);
-    vs.fetch(vb, p.v.l, 32 * t, keys, p.d, lane, kk);
-  }
+  uint32_t kept = 1u;                                       // of the next tile's key that this lane (and lane + 32) asked about
+  const auto ask = [&](int tile) {
+    const int j = 32 * tile + (lane & 31);
+    if (MASK && kk.at) kept = tile < t1 && j < keys ? kk.at[(long)j * kk.step] : 0u;
+  };
+  const auto fetch = [&](int tile) {
+    if (MASK) {
+      const KeepBits keep = {(uint32_t)__ballot(kept != 0u), 32 * tile};
+      ks.fetch(kb, p.k.l, 32 * tile, keys, p.d, lane, keep);
+      vs.fetch(vb, p.v.l, 32 * tile, keys, p.d, lane, keep);
+    } else {
+      ks.fetch(kb, p.k.l, 32 * tile, keys, p.d, lane, Keep{});
+      vs.fetch(vb, p.v.l, 32 * tile, keys, p.d, lane, Keep{});
+    }
+    ask(tile + 4);
+  };
+  ask(t);
+  if (t < t1) fetch(t);
   for (; t < t1; t += 4) {
     ks.put(kt, lane);
     vs.put(vt, lane);
-    if (t + 4 < t1) {
-      ks.fetch(kb, p.k.l, 32 * (t + 4), keys, p.d, lane, kk);
-      vs.fetch(vb, p.v.l, 32 * (t + 4), keys, p.d, lane, kk);
-    }
+    if (t + 4 < t1) fetch(t + 4);
     const int j0 = 32 * t;
     f32x16 bias;                                            // read in front of the fence: sixteen loads in flight, not one by one
     if (BIAS) {
